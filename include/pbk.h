@@ -52,6 +52,7 @@ extern "C" {
 /* dtype codes */
 #define PBK_F32 0
 #define PBK_BF16 1
+#define PBK_F16 2 /* the paged cache's keys, values and queries only */
 
 /* state layouts */
 #define PBK_STATE_KV 0 /* [.., dk, dv]: pseudobrain/gated_deltanet.py:72-75 */
@@ -637,6 +638,118 @@ PBK_API int pbk_ipc_handle(const void* ptr, void* handle, int64_t* offset);
 PBK_API int pbk_ipc_open(const void* handle, void** base);
 PBK_API int pbk_ipc_close(void* base);
 PBK_API int pbk_copy_async(void* dst, const void* src, size_t bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key-value cache: the dense single-token attention of a server's sequences over one
+ * pool of pages, and the bounded cache that evicts by accumulated attention weight.
+ *
+ * k_pages, v_pages [pages, kv, page, d]; entry i of sequence b lies in page
+ * block_table[b][i / page] at row i % page, for every key head. Beside them, per entry and
+ * key head, mass (fp32, the attention weight accumulated so far) and pos (int32, the token's
+ * position) [pages, kv, page]. Query head j reads key head j / (h / kv).
+ *
+ * lengths[b] is the number of entries that the call's comment names; it is read as 0 when
+ * negative and as block_table's capacity when above it. A page id outside the pool is never
+ * followed: its entries read as zeros and are not written. Rows of a page past a sequence's
+ * length may hold anything (NaN included): no result depends on them. A page belongs to one
+ * sequence where a call writes it (append, move, and the calls that add to mass); attention
+ * alone may read pages that several sequences share.
+ *
+ * d 64, 128 or 256; page a power of two from 8 to 256; at most 64 query heads per key head
+ * and 65535 sequences. Nothing is synchronised, and the order of every sum is fixed by the
+ * sizes and lengths: the same call gives the same bits.
+ * ------------------------------------------------------------------------ */
+typedef struct pbk_paged_cache {
+  int32_t kv, d, page, pages; /* key heads, head dim, entries per page, pages in the pool */
+  int32_t dtype;              /* keys, values and queries: PBK_BF16 or PBK_F16 */
+  int32_t pad_;
+  void* k_pages;
+  void* v_pages;              /* strides as k_pages */
+  int64_t stride_page, stride_head, stride_entry; /* elements, multiples of 8; d contiguous */
+  float* mass;                /* may be NULL where a call does not name it */
+  int32_t* pos;               /* strides as mass */
+  int64_t meta_page, meta_head; /* elements; the entries of a page are contiguous */
+} pbk_paged_cache;
+
+typedef struct pbk_paged_batch {
+  int32_t batch, width;       /* sequences; pages per row of block_table */
+  const int32_t* block_table;
+  int64_t table_stride;       /* elements between rows */
+  const int32_t* lengths;     /* [batch] */
+  const int32_t* seen;        /* [batch] tokens seen so far, those evicted included */
+} pbk_paged_batch;
+
+/* Put new tokens into the cache: token i of sequence b becomes entry lengths[b] + i (lengths
+ * before the call) with mass 0 and position seen[b] + i (mass and pos are written where the
+ * cache has them; seen NULL: lengths[b] + i). k and v are [tokens, kv, d] with one pair of
+ * strides; the tokens of sequence b are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (NULL: one
+ * token per sequence). Tokens past the table's capacity are not written. */
+PBK_API int pbk_paged_append(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const void* k, const void* v,
+                             int64_t stride_t, int64_t stride_h, int32_t tokens, const int32_t* cu_seqlens,
+                             void* stream);
+
+/* Attention of one new token per sequence over its cache: q, out [batch, h, d],
+ *   out_j = sum_i p_ji v_i,  p_j = softmax over the visible entries of scale q_j.k_i,
+ *   lse_j = log sum_i exp(scale q_j.k_i)            (natural logarithm, fp32 [batch, h])
+ * with entry i < lengths[b] visible when window <= 0, i >= lengths[b] - window or i < sinks
+ * (lengths after the token was appended; the window counts entries, so it is for a cache
+ * whose entries lie in order). A sequence without visible entries gives out 0 and lse -inf.
+ * accumulate != 0: mass_i += sum_j p_ji over the key head's query heads. Workspace bytes from
+ * pbk_paged_attend_workspace (0 for a desc that the call would reject). */
+typedef struct pbk_paged_attend_desc {
+  int32_t h, window, sinks, accumulate;
+  float scale;
+  int32_t out_dtype;          /* the cache's dtype or PBK_F32 */
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  void* out;
+  int64_t out_stride_b, out_stride_h;
+  float* lse;
+} pbk_paged_attend_desc;
+
+PBK_API size_t pbk_paged_attend_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                                          const pbk_paged_attend_desc* desc);
+PBK_API int pbk_paged_attend(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                             const pbk_paged_attend_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Add the attention weights of a sequence's last queries to mass: q [batch, queries, h, d],
+ * query w standing at entry lengths[b] - queries + w (lengths with those tokens appended);
+ * entry i is visible to it when i <= that place, and a query whose place is negative adds
+ * nothing. mass_i += sum over queries and the key head's query heads of their weights. At
+ * most 1024 queries. */
+typedef struct pbk_paged_observe_desc {
+  int32_t h, queries;
+  float scale;
+  int32_t pad_;
+  const void* q;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+} pbk_paged_observe_desc;
+
+PBK_API size_t pbk_paged_observe_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                                           const pbk_paged_observe_desc* desc);
+PBK_API int pbk_paged_observe(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                              const pbk_paged_observe_desc* desc, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* What leaves a bounded cache. For each sequence with lengths[b] > budget and each key head,
+ * `budget` entries stay: in the order protected entries (0 <= pos < sinks, or
+ * pos >= seen[b] - recent), then NaN masses, then by mass downwards (-0 is 0), ties to the
+ * lowest entry. The entries that stay and lie at or past `budget` are to move into the places
+ * below it that become free: src (those entries) and dst (those places), both ascending, the
+ * n-th to the n-th, and count [batch, kv]. src and dst are [batch, kv, moves] with moves at
+ * least min(budget, capacity - budget) (capacity = width * page; less is PBK_ERR_SHAPE); places
+ * past count hold -1. After the moves the sequence has `budget` entries, in no particular
+ * order. sinks + recent <= budget. */
+PBK_API size_t pbk_paged_select_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget);
+PBK_API int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget,
+                             int32_t recent, int32_t sinks, int32_t* src, int32_t* dst, int32_t* count, int32_t moves,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Entry dst[b][h][n] := entry src[b][h][n] (key, value, and mass and pos where the cache has
+ * them) for n < count[b][h]. The places named by dst must not be sources. Entries outside the
+ * table's capacity are left out. batch->lengths is not read. */
+PBK_API int pbk_paged_move(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const int32_t* src,
+                           const int32_t* dst, const int32_t* count, int32_t moves, void* stream);
 
 #ifdef __cplusplus
 }

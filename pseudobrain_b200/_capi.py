@@ -19,7 +19,7 @@ PBK_ERR_TIMEOUT = -7
 PBK_IPC_HANDLE_BYTES = 64
 PBK_ERR_TOO_LARGE = -9
 PBK_QUEST_NOALLOC_MAX_SCORES = 4194304
-PBK_F32, PBK_BF16 = 0, 1
+PBK_F32, PBK_BF16, PBK_F16 = 0, 1, 2
 PBK_STATE_KV, PBK_STATE_VK = 0, 1
 
 
@@ -140,7 +140,35 @@ class PbkArchiveWriteDesc(ctypes.Structure):
                 ("bnd_stride_kv", ctypes.c_int64), ("bnd_stride_p", ctypes.c_int64)]
 
 
+class PbkPagedCache(ctypes.Structure):
+    _fields_ = [("kv", ctypes.c_int32), ("d", ctypes.c_int32), ("page", ctypes.c_int32), ("pages", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("pad_", ctypes.c_int32), ("k_pages", ctypes.c_void_p),
+                ("v_pages", ctypes.c_void_p), ("stride_page", ctypes.c_int64), ("stride_head", ctypes.c_int64),
+                ("stride_entry", ctypes.c_int64), ("mass", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("meta_page", ctypes.c_int64), ("meta_head", ctypes.c_int64)]
+
+
+class PbkPagedBatch(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("width", ctypes.c_int32), ("block_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("seen", ctypes.c_void_p)]
+
+
+class PbkPagedAttendDesc(ctypes.Structure):
+    _fields_ = [("h", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("accumulate", ctypes.c_int32), ("scale", ctypes.c_float), ("out_dtype", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_stride_b", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+                ("lse", ctypes.c_void_p)]
+
+
+class PbkPagedObserveDesc(ctypes.Structure):
+    _fields_ = [("h", ctypes.c_int32), ("queries", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("pad_", ctypes.c_int32), ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64),
+                ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64)]
+
+
 _QD = ctypes.POINTER(PbkQuestDesc)
+_PC, _PB = ctypes.POINTER(PbkPagedCache), ctypes.POINTER(PbkPagedBatch)
 _QL = ctypes.POINTER(PbkQuestLevels)
 _VP, _I32, _I64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
 
@@ -196,6 +224,14 @@ SIGNATURES = {
     "pbk_quest_token_scores": (ctypes.c_int, [ctypes.POINTER(PbkTokenDesc), _VP]),
     "pbk_quest_token_rerank": (ctypes.c_int, [ctypes.POINTER(PbkTokenDesc), _VP]),
     "pbk_quest_row_ranks": (ctypes.c_int, [_VP, _I64, _I32, _I32, _VP, _I64, _VP]),
+    "pbk_paged_append": (ctypes.c_int, [_PC, _PB, _VP, _VP, _I64, _I64, _I32, _VP, _VP]),
+    "pbk_paged_attend_workspace": (ctypes.c_size_t, [_PC, _PB, ctypes.POINTER(PbkPagedAttendDesc)]),
+    "pbk_paged_attend": (ctypes.c_int, [_PC, _PB, ctypes.POINTER(PbkPagedAttendDesc), _VP, ctypes.c_size_t, _VP]),
+    "pbk_paged_observe_workspace": (ctypes.c_size_t, [_PC, _PB, ctypes.POINTER(PbkPagedObserveDesc)]),
+    "pbk_paged_observe": (ctypes.c_int, [_PC, _PB, ctypes.POINTER(PbkPagedObserveDesc), _VP, ctypes.c_size_t, _VP]),
+    "pbk_paged_select_workspace": (ctypes.c_size_t, [_PC, _PB, _I32]),
+    "pbk_paged_select": (ctypes.c_int, [_PC, _PB, _I32, _I32, _I32, _VP, _VP, _VP, _I32, _VP, ctypes.c_size_t, _VP]),
+    "pbk_paged_move": (ctypes.c_int, [_PC, _PB, _VP, _VP, _VP, _I32, _VP]),
     "pbk_ipc_handle": (ctypes.c_int, [_VP, _VP, ctypes.POINTER(ctypes.c_int64)]),
     "pbk_ipc_open": (ctypes.c_int, [_VP, ctypes.POINTER(ctypes.c_void_p)]),
     "pbk_ipc_close": (ctypes.c_int, [_VP]),

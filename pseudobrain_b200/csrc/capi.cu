@@ -3,6 +3,7 @@
 #include <cstdint>
 
 #include "common.cuh"
+#include "paged.cuh"
 #include "quest.cuh"
 #include "swa.cuh"
 
@@ -770,6 +771,158 @@ int pbk_quest_row_ranks(const float* x, int64_t x_stride, int32_t rows, int32_t 
   if (st != PBK_OK) return st;
   return launch_status(pbk::launch_quest_row_ranks(x, x_stride, rows, n, ranks, ranks_stride,
                                                    static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ paged key-value cache
+namespace {
+// `need`: 1 keys, 2 values, 4 mass, 8 pos.
+int validate_paged(const pbk_paged_cache* c, const pbk_paged_batch* b, int need, bool lengths = true) {
+  if (c == nullptr || b == nullptr) return PBK_ERR_INVALID;
+  if (c->kv < 1 || c->pages < 0 || b->batch < 0 || b->width < 0) return PBK_ERR_INVALID;
+  if (c->page < 8 || c->page > 256 || (c->page & (c->page - 1)) != 0) return PBK_ERR_SHAPE;
+  if (c->kv > 65535 || b->batch > 65535) return PBK_ERR_SHAPE;  // grid y and z
+  if ((int64_t)b->width * c->page > INT32_MAX - 65536) return PBK_ERR_SHAPE;  // entries are 32-bit
+  if (need & 3) {
+    if (c->d != 64 && c->d != 128 && c->d != 256) return PBK_ERR_SHAPE;
+    if (c->dtype != PBK_BF16 && c->dtype != PBK_F16) return PBK_ERR_DTYPE;
+  }
+  if (b->batch == 0) return PBK_OK;
+  if (c->pages > 0) {
+    if (((need & 1) && !c->k_pages) || ((need & 2) && !c->v_pages) || ((need & 4) && !c->mass) ||
+        ((need & 8) && !c->pos))
+      return PBK_ERR_INVALID;
+    if (need & 3) {
+      if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || !aligned_elems(c->stride_page, 8) ||
+          !aligned_elems(c->stride_head, 8) || !aligned_elems(c->stride_entry, 8))
+        return PBK_ERR_ALIGN;
+      if (c->stride_page <= 0 || c->stride_head <= 0 || c->stride_entry <= 0) return PBK_ERR_INVALID;
+    }
+    if ((c->mass || c->pos) && (c->meta_page <= 0 || c->meta_head <= 0)) return PBK_ERR_INVALID;
+  }
+  if ((b->width > 0 && !b->block_table) || (lengths && !b->lengths)) return PBK_ERR_INVALID;
+  if (b->table_stride < 0) return PBK_ERR_INVALID;
+  return PBK_OK;
+}
+
+int validate_attend(const pbk_paged_cache* c, const pbk_paged_batch* b, const pbk_paged_attend_desc* d) {
+  if (d == nullptr) return PBK_ERR_INVALID;
+  const int st = validate_paged(c, b, 3 | (d->accumulate ? 4 : 0));
+  if (st != PBK_OK) return st;
+  if (d->h < 1 || d->sinks < 0 || !(d->scale > 0.f)) return PBK_ERR_INVALID;
+  if (d->h % c->kv != 0 || d->h / c->kv > 64) return PBK_ERR_SHAPE;
+  if (d->out_dtype != PBK_F32 && d->out_dtype != c->dtype) return PBK_ERR_DTYPE;
+  if (b->batch == 0) return PBK_OK;
+  if (!d->q || !d->out || !d->lse) return PBK_ERR_INVALID;
+  const int64_t ev = d->out_dtype == PBK_F32 ? 4 : 8;
+  if (!aligned16(d->q) || !aligned_elems(d->q_stride_b, 8) || !aligned_elems(d->q_stride_h, 8) || !aligned16(d->out) ||
+      !aligned_elems(d->out_stride_b, ev) || !aligned_elems(d->out_stride_h, ev))
+    return PBK_ERR_ALIGN;
+  return PBK_OK;
+}
+
+int validate_observe(const pbk_paged_cache* c, const pbk_paged_batch* b, const pbk_paged_observe_desc* d) {
+  if (d == nullptr) return PBK_ERR_INVALID;
+  const int st = validate_paged(c, b, 5);
+  if (st != PBK_OK) return st;
+  if (d->h < 1 || d->queries < 0 || !(d->scale > 0.f)) return PBK_ERR_INVALID;
+  if (d->h % c->kv != 0 || d->h / c->kv > 64 || d->queries > 1024) return PBK_ERR_SHAPE;
+  if (b->batch == 0 || d->queries == 0) return PBK_OK;
+  if (!d->q) return PBK_ERR_INVALID;
+  if (!aligned16(d->q) || !aligned_elems(d->q_stride_b, 8) || !aligned_elems(d->q_stride_t, 8) ||
+      !aligned_elems(d->q_stride_h, 8))
+    return PBK_ERR_ALIGN;
+  return PBK_OK;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (need == 0) return PBK_OK;
+  if (ws == nullptr || have < need) return PBK_ERR_WORKSPACE;
+  return aligned16(ws) ? PBK_OK : PBK_ERR_ALIGN;
+}
+}  // namespace
+
+extern "C" {
+
+int pbk_paged_append(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const void* k, const void* v,
+                     int64_t stride_t, int64_t stride_h, int32_t tokens, const int32_t* cu_seqlens, void* stream) {
+  int st = validate_paged(cache, batch, 3);
+  if (st != PBK_OK) return st;
+  if (tokens < 0 || (cu_seqlens == nullptr && tokens != batch->batch)) return PBK_ERR_INVALID;
+  if (batch->batch == 0 || tokens == 0 || cache->pages == 0) return PBK_OK;
+  if (!k || !v) return PBK_ERR_INVALID;
+  if (!aligned16(k) || !aligned16(v) || !aligned_elems(stride_t, 8) || !aligned_elems(stride_h, 8)) return PBK_ERR_ALIGN;
+  if ((st = check_current_device()) != PBK_OK) return st;
+  return launch_status(pbk::launch_paged_append(*cache, *batch, k, v, stride_t, stride_h, tokens, cu_seqlens,
+                                                static_cast<cudaStream_t>(stream)));
+}
+
+size_t pbk_paged_attend_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                                  const pbk_paged_attend_desc* desc) {
+  if (validate_attend(cache, batch, desc) != PBK_OK || batch->batch == 0) return 0;
+  return pbk::paged_attend_workspace(*cache, *batch, *desc);
+}
+
+int pbk_paged_attend(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const pbk_paged_attend_desc* desc,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  int st = validate_attend(cache, batch, desc);
+  if (st != PBK_OK || batch->batch == 0) return st;
+  st = check_workspace(workspace, workspace_bytes, pbk::paged_attend_workspace(*cache, *batch, *desc));
+  if (st != PBK_OK) return st;
+  if ((st = check_current_device()) != PBK_OK) return st;
+  return launch_status(pbk::launch_paged_attend(*cache, *batch, *desc, workspace, static_cast<cudaStream_t>(stream)));
+}
+
+size_t pbk_paged_observe_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
+                                   const pbk_paged_observe_desc* desc) {
+  if (validate_observe(cache, batch, desc) != PBK_OK || batch->batch == 0 || desc->queries == 0) return 0;
+  return pbk::paged_observe_workspace(*cache, *batch, *desc);
+}
+
+int pbk_paged_observe(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const pbk_paged_observe_desc* desc,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  int st = validate_observe(cache, batch, desc);
+  if (st != PBK_OK || batch->batch == 0 || desc->queries == 0 || cache->pages == 0) return st;
+  st = check_workspace(workspace, workspace_bytes, pbk::paged_observe_workspace(*cache, *batch, *desc));
+  if (st != PBK_OK) return st;
+  if ((st = check_current_device()) != PBK_OK) return st;
+  return launch_status(pbk::launch_paged_observe(*cache, *batch, *desc, workspace, static_cast<cudaStream_t>(stream)));
+}
+
+size_t pbk_paged_select_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget) {
+  if (validate_paged(cache, batch, 12) != PBK_OK || batch->batch == 0 || budget < 1) return 0;
+  return pbk::paged_select_workspace(*cache, *batch, budget);
+}
+
+int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget, int32_t recent,
+                     int32_t sinks, int32_t* src, int32_t* dst, int32_t* count, int32_t moves, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int st = validate_paged(cache, batch, 12);
+  if (st != PBK_OK) return st;
+  if (budget < 1 || recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget || moves < 0) return PBK_ERR_INVALID;
+  if (batch->batch == 0) return PBK_OK;
+  const int64_t past = (int64_t)batch->width * cache->page - budget;
+  if (moves < (past < budget ? past : budget)) return PBK_ERR_SHAPE;
+  if (!batch->seen || !count || (moves > 0 && (!src || !dst))) return PBK_ERR_INVALID;
+  st = check_workspace(workspace, workspace_bytes, pbk::paged_select_workspace(*cache, *batch, budget));
+  if (st != PBK_OK) return st;
+  if ((st = check_current_device()) != PBK_OK) return st;
+  return launch_status(pbk::launch_paged_select(*cache, *batch, budget, recent, sinks, src, dst, count, moves, workspace,
+                                                static_cast<cudaStream_t>(stream)));
+}
+
+int pbk_paged_move(const pbk_paged_cache* cache, const pbk_paged_batch* batch, const int32_t* src, const int32_t* dst,
+                   const int32_t* count, int32_t moves, void* stream) {
+  int st = validate_paged(cache, batch, 3, false);
+  if (st != PBK_OK) return st;
+  if (moves < 0) return PBK_ERR_INVALID;
+  if (batch->batch == 0 || moves == 0 || cache->pages == 0) return PBK_OK;
+  if (!src || !dst || !count) return PBK_ERR_INVALID;
+  if ((int64_t)moves * (cache->d / 8) > INT32_MAX) return PBK_ERR_SHAPE;
+  if ((st = check_current_device()) != PBK_OK) return st;
+  return launch_status(pbk::launch_paged_move(*cache, *batch, src, dst, count, moves,
+                                              static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,54 @@
+// The paged key-value cache: addressing shared by its kernels, and their launchers (called
+// by the C ABI after validation).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/pbk.h"
+
+namespace pbk {
+
+#ifdef __CUDACC__
+namespace paged {
+
+// Entries of sequence b that the table can hold (lengths outside [0, capacity] are clamped).
+__device__ __forceinline__ int clamp_length(int n, int width, int page) {
+  const int64_t cap = (int64_t)width * page;
+  return n < 0 ? 0 : (n > cap ? (int)cap : n);
+}
+
+// Pool page of entry j of table row `row`, -1 when the id lies outside the pool.
+__device__ __forceinline__ int page_of(const int32_t* row, int j, int log_page, int pages) {
+  const int id = row[j >> log_page];
+  return (unsigned)id < (unsigned)pages ? id : -1;
+}
+
+}  // namespace paged
+#endif
+
+inline int paged_log2(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+
+cudaError_t launch_paged_append(const pbk_paged_cache& c, const pbk_paged_batch& b, const void* k, const void* v,
+                                int64_t stride_t, int64_t stride_h, int tokens, const int32_t* cu_seqlens,
+                                cudaStream_t st);
+size_t paged_attend_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_attend_desc& d);
+cudaError_t launch_paged_attend(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_attend_desc& d,
+                                void* ws, cudaStream_t st);
+size_t paged_observe_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d);
+cudaError_t launch_paged_observe(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d,
+                                 void* ws, cudaStream_t st);
+size_t paged_select_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget);
+cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
+                                int32_t* src, int32_t* dst, int32_t* count, int moves, void* ws, cudaStream_t st);
+cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
+                              const int32_t* dst, const int32_t* count, int moves, cudaStream_t st);
+
+}  // namespace pbk

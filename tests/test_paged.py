@@ -1,0 +1,130 @@
+"""The paged cache without a GPU: the C ABI's structures and refusals, and the oracle against
+the sliding-window oracle."""
+from __future__ import annotations
+
+import ctypes
+import os
+import subprocess
+import tempfile
+
+import numpy as np
+import pytest
+
+from oracle import paged as op
+from oracle import swa as oswa
+from tests.conftest import ROOT
+
+FAKE = 1 << 20  # 16-byte aligned, never dereferenced
+
+
+@pytest.fixture(scope="module")
+def capi():
+    from pseudobrain_b200 import build
+    build.build()
+    from pseudobrain_b200 import _capi
+    return _capi
+
+
+@pytest.mark.parametrize("cname,pyname", [("pbk_paged_cache", "PbkPagedCache"), ("pbk_paged_batch", "PbkPagedBatch"),
+                                          ("pbk_paged_attend_desc", "PbkPagedAttendDesc"),
+                                          ("pbk_paged_observe_desc", "PbkPagedObserveDesc")])
+def test_descriptor_layout_matches_header(capi, cname, pyname):
+    cls = getattr(capi, pyname)
+    fields = [f for f, _ in cls._fields_]
+    src = "#include <stdio.h>\n#include <stddef.h>\n#include \"pbk.h\"\nint main(void){\n"
+    src += "".join(f'printf("%zu\\n", offsetof({cname}, {f}));\n' for f in fields)
+    src += f'printf("%zu\\n", sizeof({cname})); return 0; }}\n'
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = os.path.join(d, "p.c"), os.path.join(d, "p")
+        with open(c, "w") as f:
+            f.write(src)
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe], check=True)
+        got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [getattr(cls, f).offset for f in fields] + [ctypes.sizeof(cls)]
+
+
+def _cache(capi, **over):
+    f = dict(kv=2, d=128, page=16, pages=10, dtype=capi.PBK_BF16, k_pages=FAKE, v_pages=FAKE, stride_page=4096,
+             stride_head=2048, stride_entry=128, mass=FAKE, pos=FAKE, meta_page=32, meta_head=16)
+    return capi.PbkPagedCache(**{**f, **over})
+
+
+def _batch(capi, **over):
+    return capi.PbkPagedBatch(**{**dict(batch=3, width=5, block_table=FAKE, table_stride=5, lengths=FAKE, seen=FAKE),
+                                 **over})
+
+
+def _attend(capi, **over):
+    f = dict(h=8, window=0, sinks=0, accumulate=0, scale=0.1, out_dtype=capi.PBK_BF16, q=FAKE, q_stride_b=1024,
+             q_stride_h=128, out=FAKE, out_stride_b=1024, out_stride_h=128, lse=FAKE)
+    return capi.PbkPagedAttendDesc(**{**f, **over})
+
+
+@pytest.mark.parametrize("where,over,status", [
+    ("cache", {"page": 12}, "SHAPE"), ("cache", {"page": 4}, "SHAPE"), ("cache", {"page": 512}, "SHAPE"),
+    ("cache", {"d": 96}, "SHAPE"), ("cache", {"dtype": 0}, "DTYPE"), ("cache", {"kv": 0}, "INVALID"),
+    ("cache", {"kv": 3}, "SHAPE"), ("cache", {"k_pages": None}, "INVALID"), ("cache", {"v_pages": FAKE + 2}, "ALIGN"),
+    ("cache", {"stride_entry": 130}, "ALIGN"), ("cache", {"stride_head": 0}, "INVALID"),
+    ("batch", {"batch": -1}, "INVALID"), ("batch", {"batch": 65536}, "SHAPE"), ("batch", {"lengths": None}, "INVALID"),
+    ("batch", {"block_table": None}, "INVALID"), ("batch", {"width": 1 << 28}, "SHAPE"),
+    ("desc", {"h": 130}, "SHAPE"), ("desc", {"h": 0}, "INVALID"), ("desc", {"sinks": -1}, "INVALID"),
+    ("desc", {"scale": 0.0}, "INVALID"), ("desc", {"scale": float("nan")}, "INVALID"),
+    ("desc", {"out_dtype": 2}, "DTYPE"), ("desc", {"q": None}, "INVALID"), ("desc", {"lse": None}, "INVALID"),
+    ("desc", {"q_stride_h": 129}, "ALIGN"), ("desc", {"out": FAKE + 4}, "ALIGN"),
+])
+def test_attend_refuses_on_the_host(capi, where, over, status):
+    c, b, d = _cache(capi), _batch(capi), _attend(capi)
+    for k, v in over.items():
+        setattr({"cache": c, "batch": b, "desc": d}[where], k, v)
+    want = getattr(capi, f"PBK_ERR_{status}")
+    assert capi.LIB.pbk_paged_attend_workspace(c, b, d) == 0
+    assert capi.LIB.pbk_paged_attend(c, b, d, FAKE, 1 << 40, None) == want
+
+
+def test_the_other_calls_refuse_on_the_host(capi):
+    L = capi.LIB
+    c, b = _cache(capi), _batch(capi)
+    o = capi.PbkPagedObserveDesc(8, 16, 0.1, 0, FAKE, 8192, 1024, 128)
+    assert L.pbk_paged_observe(_cache(capi, mass=None), b, o, FAKE, 1 << 40, None) == capi.PBK_ERR_INVALID
+    o.queries = 1025
+    assert L.pbk_paged_observe(c, b, o, FAKE, 1 << 40, None) == capi.PBK_ERR_SHAPE
+    assert L.pbk_paged_append(c, b, FAKE, FAKE, 256, 128, 4, None, None) == capi.PBK_ERR_INVALID  # 4 tokens, 3 sequences
+    assert L.pbk_paged_append(c, b, FAKE, FAKE + 8, 256, 128, 3, None, None) == capi.PBK_ERR_ALIGN
+    sel = lambda budget, recent, sinks, moves, cc=c, bb=b: L.pbk_paged_select(  # noqa: E731
+        cc, bb, budget, recent, sinks, FAKE, FAKE, FAKE, moves, FAKE, 1 << 40, None)
+    assert sel(32, 30, 3, 32) == capi.PBK_ERR_INVALID     # more protected than kept
+    assert sel(0, 0, 0, 32) == capi.PBK_ERR_INVALID
+    assert sel(32, 0, 0, 31) == capi.PBK_ERR_SHAPE        # capacity 80, budget 32: 32 moves
+    assert sel(64, 0, 0, 15) == capi.PBK_ERR_SHAPE        # 16 moves
+    assert sel(32, 0, 0, 32, _cache(capi, pos=None)) == capi.PBK_ERR_INVALID
+    assert sel(32, 0, 0, 32, c, _batch(capi, seen=None)) == capi.PBK_ERR_INVALID
+    assert L.pbk_paged_move(c, b, FAKE, None, FAKE, 3, None) == capi.PBK_ERR_INVALID
+    none = _batch(capi, batch=0)
+    assert L.pbk_paged_attend(c, none, _attend(capi), None, 0, None) == capi.PBK_OK
+    assert L.pbk_paged_move(c, none, FAKE, FAKE, FAKE, 3, None) == capi.PBK_OK
+    assert sel(32, 0, 0, 32, c, none) == capi.PBK_OK
+
+
+def test_module_imports_and_refuses_cpu_tensors(capi):
+    import torch
+    from pseudobrain_b200 import paged_cache as P
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.PagedCache(torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16), torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 3), (1, 0)])
+def test_oracle_attention_is_the_last_row_of_the_window_oracle(window, sinks):
+    rng = np.random.default_rng(0)
+    b, h, kv, n, d, page = 2, 6, 2, 45, 64, 8
+    k, v = rng.standard_normal((2, b, kv, n, d))
+    q = rng.standard_normal((b, h, n, d))
+    table = rng.permutation(b * 6).reshape(b, 6)
+    kp, vp = np.full((2, b * 6, kv, page, d), np.nan)
+    for i in range(b):
+        p, r = op.entry(table, page, i, np.arange(n))
+        kp[p, :, r], vp[p, :, r] = k[i].transpose(1, 0, 2), v[i].transpose(1, 0, 2)
+    out, lse, w = op.attend(q[:, :, -1], kp, vp, table, [n, n], window, sinks)
+    assert np.allclose(out, oswa.causal_attention(q, k, v, window, sinks)[:, :, -1], atol=1e-12)
+    assert np.allclose([x.sum() for x in w], h)
+    if window is None:
+        assert np.allclose(op.observe(q[:, :, -1:].transpose(0, 2, 1, 3), kp, table, [n, n]), w, atol=1e-12)
