@@ -668,7 +668,7 @@ typedef struct pbk_paged_cache {
   int64_t stride_page, stride_head, stride_entry; /* elements, multiples of 8; d contiguous */
   float* mass;                /* may be NULL where a call does not name it */
   int32_t* pos;               /* strides as mass */
-  int64_t meta_page, meta_head; /* elements; the entries of a page are contiguous */
+  int64_t meta_page, meta_head; /* elements, multiples of 4; the entries of a page are contiguous */
 } pbk_paged_cache;
 
 typedef struct pbk_paged_batch {

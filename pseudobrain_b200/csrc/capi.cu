@@ -783,6 +783,7 @@ int validate_paged(const pbk_paged_cache* c, const pbk_paged_batch* b, int need,
   if (c->kv < 1 || c->pages < 0 || b->batch < 0 || b->width < 0) return PBK_ERR_INVALID;
   if (c->page < 8 || c->page > 256 || (c->page & (c->page - 1)) != 0) return PBK_ERR_SHAPE;
   if (c->kv > 65535 || b->batch > 65535) return PBK_ERR_SHAPE;  // grid y and z
+  if ((int64_t)c->kv * b->batch > INT32_MAX / 256) return PBK_ERR_SHAPE;  // (sequence, head) pairs, query heads: grid x
   if ((int64_t)b->width * c->page > INT32_MAX - 65536) return PBK_ERR_SHAPE;  // entries are 32-bit
   if (need & 3) {
     if (c->d != 64 && c->d != 128 && c->d != 256) return PBK_ERR_SHAPE;
@@ -800,6 +801,8 @@ int validate_paged(const pbk_paged_cache* c, const pbk_paged_batch* b, int need,
       if (c->stride_page <= 0 || c->stride_head <= 0 || c->stride_entry <= 0) return PBK_ERR_INVALID;
     }
     if ((c->mass || c->pos) && (c->meta_page <= 0 || c->meta_head <= 0)) return PBK_ERR_INVALID;
+    if (!aligned16(c->mass) || !aligned16(c->pos) || !aligned_elems(c->meta_page, 4) || !aligned_elems(c->meta_head, 4))
+      return PBK_ERR_ALIGN;
   }
   if ((b->width > 0 && !b->block_table) || (lengths && !b->lengths)) return PBK_ERR_INVALID;
   if (b->table_stride < 0) return PBK_ERR_INVALID;

@@ -7,7 +7,11 @@
 // walks its run with an online softmax (base 2) and writes a head's result when its run holds
 // the whole head, else the partial (maximum, sum, weighted values) of its piece; the join
 // kernel, launched behind it, merges the pieces of each head and, when asked, turns the scores
-// kept in the workspace into weights and adds them to the cache's mass.
+// kept in the workspace into weights and adds them to the cache's mass. Few short heads take
+// the other way: one CTA per head, whose warps share its units and join in shared memory, one
+// launch in all (see `whole_heads`).
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "tc.cuh"
@@ -19,12 +23,14 @@ namespace {
 constexpr int kUnit = 16;           // entries per unit
 constexpr int kRing = 192 * 1024;   // staging bytes per CTA
 constexpr int kMinUnits = 2;        // units per warp below which fewer warps take part
+constexpr int kWholeUnits = 128;    // most units per head where one CTA takes a whole head
 constexpr int kJoinThreads = 256;
-constexpr int kSlice = 2048;        // entries per CTA of the mass update
+constexpr int kMassThreads = 256;
+constexpr int kPad = 4;             // floats after a partial row's D values: maximum, sum, two unused
 
 template <int D>
 struct Shape {
-  static constexpr int kWarps = D == 256 ? 4 : 8;
+  static constexpr int kWarps = D == 256 ? 6 : 8;
   static constexpr int kTile = kUnit * D * 2;  // bytes of a unit's keys (or values)
   static constexpr int kStages = kRing / (kWarps * 2 * kTile);
 };
@@ -48,10 +54,12 @@ struct AttendArgs {
   int pages;
   // workspace
   int64_t* base;             // [batch + 1] units of the sequences before, per (head, row tile)
-  float* part;               // [warps][2][rows][D + 2]
-  float* lse2;               // [batch, h] base 2, of the heads that one warp held whole
-  float* scores;             // [units][16][score_stride] base 2
-  int score_stride, d;
+  int4* open;                // [runs] the head that a run begins and does not end: its sequence (-1:
+                             // none), its index among the sequence's heads and row tiles, the run that ends it
+  float* part;               // [runs][2][rows][D + kPad]
+  float* lse2;               // [batch, h] base 2
+  float* scores;             // [units][rows][16] base 2
+  int64_t whole_units;       // score units set apart per head where a CTA takes a whole head
   int* err;
 };
 
@@ -130,20 +138,66 @@ struct Span {
   __device__ int entry(int t) const { return (t < sink_units ? t : first + t - sink_units) * kUnit; }
 };
 
-__device__ __forceinline__ int64_t run_start(int64_t total, int warps, int w) { return total * w / warps; }
-// The warp whose run holds unit u.
-__device__ __forceinline__ int run_of(int64_t total, int warps, int64_t u) {
-  return (int)(((u + 1) * warps - 1) / total);
+// Units per run: equal for all but the last run, at least kMinUnits.
+__device__ __forceinline__ int run_length(int64_t total, int warps) {
+  const int64_t x = total + warps - 1;
+  const int64_t len = (x >> 32) == 0 ? (uint32_t)x / (uint32_t)warps : x / warps;
+  return max((int)len, kMinUnits);
 }
-__device__ __forceinline__ int active_warps(int64_t total, int warps) {
-  const int64_t w = (total + kMinUnits - 1) / kMinUnits;
-  return w < warps ? (w > 0 ? (int)w : 1) : warps;
+// The run that holds unit u.
+__device__ __forceinline__ int run_of(int64_t u, int length) {
+  return (u >> 32) == 0 ? (int)((uint32_t)u / (uint32_t)length) : (int)(u / length);
 }
 
-__device__ __forceinline__ void store_out(const AttendArgs& a, bool f16, int64_t at, float y) {
+constexpr float kLn2 = 0.6931471805599453f;
+
+// The sum over the 8 lanes that hold a query row's entries.
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+
+template <bool F16>
+__device__ __forceinline__ void store_out(const AttendArgs& a, int64_t at, float y) {
   if (a.out_f32) static_cast<float*>(a.out)[at] = y;
-  else if (f16) static_cast<__half*>(a.out)[at] = __float2half_rn(y);
+  else if (F16) static_cast<__half*>(a.out)[at] = __float2half_rn(y);
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
+}
+
+// Adds the weights of quarter i (four entries; i / 4 counts the head's units) of one (sequence,
+// key head) to their mass: one page id, one 16-byte access to the mass and one to each row's
+// scores serve them. `scores` are those of the head's first unit in the first row tile, `tile`
+// floats from one row tile's to the next's; lse2[r] the rows' logarithms (INFINITY for a row
+// without weight: it adds 0).
+__device__ __forceinline__ void add_weights(const AttendArgs& a, int b, int h, const Span& s, int i,
+                                            const float* scores, int64_t tile, const float* lse2) {
+  const int e = s.entry(i / 4) + i % 4 * 4;
+  if (e >= s.n) return;
+  const int page = a.table[b * a.table_stride + (e >> a.log_page)];
+  const float* x = scores + (int64_t)(i / 4) * (kUnit * a.rows) + i % 4 * 4;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r0 = 0; r0 < a.groups; r0 += a.rows, x += tile) {
+    const int rows = min(a.rows, a.groups - r0);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const float4 y = *reinterpret_cast<const float4*>(x + r * kUnit);
+      const float l = lse2[r0 + r];
+      sum.x += ex2(y.x - l), sum.y += ex2(y.y - l), sum.z += ex2(y.z - l), sum.w += ex2(y.w - l);
+    }
+  }
+  if ((unsigned)page >= (unsigned)a.pages) return;
+  float4* to = reinterpret_cast<float4*>(a.mass + page * a.meta_page + h * a.meta_head + (e & (a.page - 1)));
+  if (e + 4 <= s.n) {
+    float4 y = *to;
+    y.x += sum.x, y.y += sum.y, y.z += sum.z, y.w += sum.w;
+    *to = y;
+  } else {  // the sequence's last entries; rows past them are left alone
+    float* f = reinterpret_cast<float*>(to);
+    f[0] += sum.x;
+    if (e + 1 < s.n) f[1] += sum.y;
+    if (e + 2 < s.n) f[2] += sum.z;
+  }
 }
 
 // Keys are the M of both products and the query rows their N: S^T = K Q^T (A = 16 keys by
@@ -161,7 +215,7 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, bool f16, int64_t
 // Weights enter the product with V as 16-bit numbers: fp16 as one (11 bits), bf16 as two (the
 // rounded weight and what the rounding left, 16 bits together), so that the result's own
 // rounding is the largest error; the second product runs in the tensor cores' idle time.
-template <int D, int NT, bool F16>
+template <int D, int NT, bool F16, bool WHOLE>
 __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     paged_attend_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                         const AttendArgs a) {
@@ -171,83 +225,88 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t s_full[S::kWarps][S::kStages];
-  __shared__ int64_t s_sum[S::kWarps];
-  __shared__ int64_t s_off[S::kWarps];
+  __shared__ int64_t s_sum[S::kWarps], s_off[S::kWarps];
   __shared__ int s_seq[S::kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nwarps = gridDim.x * S::kWarps;
   const int pairs = a.kv * a.rt;  // (key head, row tile) of a sequence
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  // ---- where each warp's run starts: a scan of the sequences' units by the whole CTA
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += Span(a, b).units;
-  int64_t before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
+  if (tid == 0) {
+    tc::prefetch_tmap(&mk);
+    tc::prefetch_tmap(&mv);
   }
-  if (lane == 31) s_sum[warp] = before;
-  if (lane < S::kStages) tc::mbar_init(&s_full[warp][lane], 1);
+
   if (lane == 0) {
-    s_seq[warp] = -1;
+    for (int i = 0; i < S::kStages; ++i) tc::mbar_init(&s_full[warp][i], 1);
     tc::fence_barrier_init();
   }
-  __syncthreads();
-  int64_t total = 0;
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < S::kWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
-  if (blockIdx.x == 0) {
-    int64_t at = before;
-    for (int b = b0; b < b1; ++b) {
-      a.base[b] = at;
-      at += Span(a, b).units;
-    }
-    if (tid == 0) a.base[a.batch] = total;
-  }
-  total *= pairs;
-  const int active = active_warps(total, nwarps);
-  if (total > 0) {
-    int64_t at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int64_t len = Span(a, b).units;
-#pragma unroll
-      for (int w = 0; w < S::kWarps; ++w) {
-        const int run = w * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs
-        if (run < active) {
-          const int64_t u = run_start(total, active, run);
-          if (u >= at * pairs && u < (at + len) * pairs) s_seq[w] = b, s_off[w] = u - at * pairs;
-        }
-      }
-      at += len;
-    }
-  }
-  __syncthreads();
-  if (s_seq[warp] < 0) return;
-  const int run = warp * gridDim.x + blockIdx.x;
-  const int64_t u0 = run_start(total, active, run);
-  const int count = (int)(run_start(total, active, run + 1) - u0);
+  __syncwarp();
 
-  // ---- producer and consumer positions in the line of units
   struct Walk {
     int b, pair, t;
     Span s;
   };
   Walk c;
-  c.b = s_seq[warp];
-  c.s = Span(a, c.b);
-  c.pair = (int)(s_off[warp] / c.s.units);
-  c.t = (int)(s_off[warp] % c.s.units);
+  int64_t u0 = 0;  // the run's first unit in the line (WHOLE: among the scores set apart)
+  int run = 0, length = 0, count;
+  if (WHOLE) {
+    c.b = blockIdx.x / pairs;
+    c.pair = blockIdx.x % pairs;
+    c.s = Span(a, c.b);
+    c.t = c.s.units * warp / S::kWarps;
+    count = c.s.units * (warp + 1) / S::kWarps - c.t;
+    u0 = blockIdx.x * a.whole_units + c.t;
+  } else {
+    // ---- where each warp's run starts: a scan of the sequences' units by the whole CTA
+    const int per = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += Span(a, b).units;
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    before -= mine;
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w];
+    }
+    length = run_length(total * pairs, nwarps);
+    int64_t at = before;
+    for (int b = b0; b < b1; ++b) {
+      const Span s(a, b);
+      if (blockIdx.x == 0) a.base[b] = at;
+      const int64_t from = at * pairs, to = from + (int64_t)s.units * pairs;
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w) {
+        const int64_t u = (int64_t)(w * gridDim.x + blockIdx.x) * length;
+        if (u >= from && u < to) s_seq[w] = b, s_off[w] = u - from;
+      }
+      at += s.units;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.base[a.batch] = total;
+    __syncthreads();
+    run = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs
+    u0 = (int64_t)run * length;
+    count = (int)max((int64_t)0, min((int64_t)length, total * pairs - u0));
+    if (lane == 0) a.open[run] = make_int4(-1, 0, 0, 0);
+    if (count == 0) return;
+    c.b = s_seq[warp];
+    c.s = Span(a, c.b);
+    c.pair = run_of(s_off[warp], c.s.units);
+    c.t = (int)(s_off[warp] - (int64_t)c.pair * c.s.units);
+  }
+
+  // ---- the producer's position (p) runs ahead of the consumer's (c)
   Walk p = c;
   auto advance = [&](Walk& w) {
-    if (++w.t < w.s.units) return;
+    if (++w.t < w.s.units || WHOLE) return;
     w.t = 0;
     if (++w.pair < pairs) return;
     w.pair = 0;
@@ -258,7 +317,7 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   };
   const bool small = a.page < kUnit;  // pages of 8: two per unit
   auto page_ids = [&](const Walk& w) {
-    if (w.b >= a.batch) return make_int2(-1, -1);
+    if (w.b >= a.batch || w.t >= w.s.units) return make_int2(-1, -1);
     const int32_t* row = a.table + w.b * a.table_stride;
     const int i = w.s.entry(w.t) >> a.log_page;
     return make_int2(row[i], small && i + 1 < a.width ? row[i + 1] : -1);
@@ -297,7 +356,15 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   uint32_t qb[NT][kK][2];
   float o[NT][kK][4];
   float m[NT][2], l[NT][2];
-  int rows = 0;
+  if (WHOLE) {  // a warp without units joins an empty part
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int kk = 0; kk < kK; ++kk) o[nt][kk][0] = o[nt][kk][1] = o[nt][kk][2] = o[nt][kk][3] = 0.f;
+  }
+  int rows = min(a.rows, a.groups);
   bool fresh = true, ok = true;
   int begun = c.t;  // first unit of the current piece in its head
   int stage = 0;
@@ -398,13 +465,15 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
       }
     }
     if (a.accumulate) {
-      float* to = a.scores + (u0 + i) * (int64_t)(kUnit * a.score_stride);
+      float* to = a.scores + (u0 + i) * (int64_t)(kUnit * a.rows) + g;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        if (8 * nt + 2 * t4 < a.score_stride) {
-          *reinterpret_cast<float2*>(to + g * a.score_stride + 8 * nt + 2 * t4) = make_float2(sc[nt][0], sc[nt][1]);
-          *reinterpret_cast<float2*>(to + (g + 8) * a.score_stride + 8 * nt + 2 * t4) = make_float2(sc[nt][2], sc[nt][3]);
-        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (8 * nt + 2 * t4 + r < rows) {
+            to[(8 * nt + 2 * t4 + r) * kUnit] = sc[nt][r];
+            to[(8 * nt + 2 * t4 + r) * kUnit + 8] = sc[nt][2 + r];
+          }
     }
     if (__any_sync(0xffffffffu, raised)) {
 #pragma unroll
@@ -436,17 +505,18 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     if (++stage == S::kStages) stage = 0, parity ^= 1;
 
     const bool ends = c.t + 1 == c.s.units;
-    if (ends || i + 1 == count) {  // the piece is complete
+    if (!WHOLE && (ends || i + 1 == count)) {  // the piece is complete
       const bool is_whole = ends && begun == 0;
-      float* pp = a.part + ((int64_t)run * 2 + (begun == 0 ? 1 : 0)) * a.rows * (D + 2);
+      float* pp = a.part + ((int64_t)run * 2 + (begun == 0 ? 1 : 0)) * a.rows * (D + kPad);
+      if (!ends && begun == 0 && lane == 0) {
+        const int64_t end = u0 + i + (c.s.units - 1 - c.t);  // the head's last unit
+        a.open[run] = make_int4(c.b, c.pair, run_of(end, length), 0);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float sum = l[nt][r];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const float sum = column_sum(l[nt][r]);
           const int row = 8 * nt + 2 * t4 + r;
           if (row >= rows) continue;
           const int j = h * a.groups + r0 + row;
@@ -455,16 +525,16 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
             const int64_t to = c.b * a.out_sb + j * a.out_sh;
 #pragma unroll
             for (int kk = 0; kk < kK; ++kk) {
-              store_out(a, F16, to + 16 * kk + g, o[nt][kk][r] * inv);
-              store_out(a, F16, to + 16 * kk + 8 + g, o[nt][kk][2 + r] * inv);
+              store_out<F16>(a, to + 16 * kk + g, o[nt][kk][r] * inv);
+              store_out<F16>(a, to + 16 * kk + 8 + g, o[nt][kk][2 + r] * inv);
             }
             if (g == 0) {
               const float lse2 = finite(m[nt][r]) - a.offset + log2f(sum);
-              a.lse[(int64_t)c.b * a.kv * a.groups + j] = lse2 * 0.6931471805599453f;
+              a.lse[(int64_t)c.b * a.kv * a.groups + j] = lse2 * kLn2;
               a.lse2[(int64_t)c.b * a.kv * a.groups + j] = lse2;
             }
           } else {
-            float* to = pp + row * (D + 2);
+            float* to = pp + row * (D + kPad);
 #pragma unroll
             for (int kk = 0; kk < kK; ++kk) {
               to[16 * kk + g] = o[nt][kk][r];
@@ -479,128 +549,182 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   }
   if (!ok)  // loads in flight land before the CTA's shared memory is given up
     for (int s = 0; s < S::kStages; ++s) tc::mbar_wait(&s_full[warp][s], parity, 200000000ull);
-}
+  if (!WHOLE) return;
 
-// The pieces of one (sequence, key head, row tile): runs first .. last, the first one's in its
-// slot 1, the others' in slot 0.
-struct Pieces {
-  int first, last;
-  __device__ Pieces(const AttendArgs& a, int64_t base, int units, int pair, int64_t total, int active) {
-    const int64_t u = base * (a.kv * a.rt) + (int64_t)pair * units;
-    first = run_of(total, active, u);
-    last = run_of(total, active, u + units - 1);
-  }
-  __device__ const float* at(const AttendArgs& a, int run, int row) const {
-    return a.part + (((int64_t)run * 2 + (run == first ? 1 : 0)) * a.rows + row) * (a.d + 2);
-  }
-};
-
-// (maximum, sum of exponentials) over the pieces, the same in every lane of the warp.
-__device__ __forceinline__ float2 join_row(const AttendArgs& a, const Pieces& pc, int row, int lane) {
-  float top = -INFINITY;
-  for (int i = pc.first + lane; i <= pc.last; i += 32) top = fmaxf(top, pc.at(a, i, row)[a.d]);
+  // ---- WHOLE: the warps' parts, each in its own (now free) ring, joined by the CTA
+  float* mine = reinterpret_cast<float*>(my_ring);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f;
-  for (int i = pc.first + lane; i <= pc.last; i += 32) {
-    const float* x = pc.at(a, i, row) + a.d;
-    sum += x[1] * ex2(x[0] - finite(top));
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float sum = column_sum(l[nt][r]);
+      float* to = mine + (8 * nt + 2 * t4 + r) * (D + kPad);
+#pragma unroll
+      for (int kk = 0; kk < kK; ++kk) {
+        to[16 * kk + g] = o[nt][kk][r];
+        to[16 * kk + 8 + g] = o[nt][kk][2 + r];
+      }
+      if (g == 0) to[D] = m[nt][r], to[D + 1] = sum;
+    }
+  __syncthreads();
+  __shared__ float s_lse[16];
+  const int h = c.pair;
+  auto part = [&](int w, int row) {
+    return reinterpret_cast<const float*>(ring + w * S::kStages * 2 * S::kTile) + row * (D + kPad);
+  };
+  for (int i = tid; i < rows * D; i += kThreads) {
+    const int row = i / D, d = i % D, j = h * a.groups + row;
+    float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, part(w, row)[D]);
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) {
+      const float f = ex2(part(w, row)[D] - finite(top));
+      sum += part(w, row)[D + 1] * f;
+      y += part(w, row)[d] * f;
+    }
+    store_out<F16>(a, c.b * a.out_sb + j * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
+    if (d == 0) {
+      const float lse2 = finite(top) - a.offset + log2f(sum);
+      a.lse[(int64_t)c.b * a.kv * a.groups + j] = lse2 * kLn2;
+      s_lse[row] = lse2 == -INFINITY ? INFINITY : lse2;  // a row without weight adds 0
+    }
   }
-  return make_float2(top, warp_sum(sum));
+  if (!a.accumulate) return;
+  __syncthreads();
+  for (int i = tid; i < 4 * c.s.units; i += kThreads)
+    add_weights(a, c.b, h, c.s, i, a.scores + blockIdx.x * a.whole_units * (kUnit * a.rows), 0, s_lse);
 }
 
-// Blocks below batch * h join the pieces of one query head; the others add the weights of kSlice
-// entries of one (sequence, key head) to the mass, from the scores in the workspace.
+// Joins the heads that no run held whole: the warps of a block share a head's rows and each
+// row's pieces (the first run's in its slot 1, the others' in slot 0), rescale as they go and
+// meet in shared memory. Where there are fewer query heads than runs (few sequences, many pieces
+// each) block i takes query head i, all warps on its one row; else (many sequences, few pieces)
+// block i looks at run i and takes the key head that it begins and does not end, if any.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kJoinThreads)
-    paged_join_kernel(const AttendArgs a, int nwarps, int slices) {
+    paged_join_kernel(const AttendArgs a, int nwarps, bool by_head) {
   constexpr int kWarps = kJoinThreads / 32;
+  constexpr int kEach = 4;  // pieces in flight per warp
   __shared__ float s_o[kWarps][D];
-  __shared__ float s_lse[64];
+  __shared__ float s_ml[kWarps][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int heads = a.kv * a.groups;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t total = a.base[a.batch] * (a.kv * a.rt);
-  const int active = active_warps(total, nwarps);
-  int64_t id = blockIdx.x;
-  if (id < (int64_t)a.batch * heads) {
-    const int b = (int)(id / heads), j = (int)(id % heads);
+  int b, h, r0, begin, end, run, last;  // key head h, row tile from r0 on, its rows [begin, end); first and last run
+  if (by_head) {
+    b = blockIdx.x / (a.kv * a.groups);
+    const int j = blockIdx.x % (a.kv * a.groups), g = j % a.groups;
+    h = j / a.groups, r0 = g / a.rows * a.rows, begin = g - r0, end = begin + 1;
     const Span s(a, b);
-    const int64_t to = b * a.out_sb + j * a.out_sh;
+    const int64_t total = a.base[a.batch] * (a.kv * a.rt);
+    const int64_t u = a.base[b] * (a.kv * a.rt) + (int64_t)(h * a.rt + g / a.rows) * s.units;
     if (s.units == 0) {
-      for (int d = tid; d < D; d += kJoinThreads) store_out(a, F16, to + d, 0.f);
-      if (tid == 0) a.lse[id] = -INFINITY;
+      for (int d = tid; d < D; d += kJoinThreads) store_out<F16>(a, b * a.out_sb + j * a.out_sh + d, 0.f);
+      if (tid == 0) a.lse[(int64_t)b * a.kv * a.groups + j] = -INFINITY;
       return;
     }
-    const int h = j / a.groups, r = j % a.groups, pair = h * a.rt + r / a.rows, row = r % a.rows;
-    const Pieces pc(a, a.base[b], s.units, pair, total, active);
-    if (pc.first == pc.last) return;  // one warp held it whole
-    const float2 ms = join_row(a, pc, row, lane);
-    const float inv = ms.y == 0.f ? 0.f : 1.f / ms.y;
+    const int length = run_length(total, nwarps);
+    run = run_of(u, length), last = run_of(u + s.units - 1, length);
+    if (run == last) return;
+  } else {
+    run = blockIdx.x;
+    const int4 open = a.open[run];
+    for (b = run; b < a.batch; b += gridDim.x)  // a sequence without entries is in no run
+      if (Span(a, b).units == 0)
+        for (int i = tid; i < a.kv * a.groups * D; i += kJoinThreads) {
+          store_out<F16>(a, b * a.out_sb + i / D * a.out_sh + i % D, 0.f);
+          if (i % D == 0) a.lse[(int64_t)b * a.kv * a.groups + i / D] = -INFINITY;
+        }
+    if (open.x < 0) return;
+    b = open.x, h = open.y / a.rt, r0 = open.y % a.rt * a.rows, last = open.z;
+    begin = 0, end = min(a.rows, a.groups - r0);
+  }
+  for (int row0 = begin; row0 < end; row0 += kWarps) {
+    const int n = min(end - row0, kWarps), each = kWarps / n;  // rows of this turn, warps per row
+    const int row = row0 + warp / each, part = warp % each;
     float acc[D / 32];
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-    for (int i = pc.first + warp; i <= pc.last; i += kWarps) {
-      const float* x = pc.at(a, i, row);
-      const float f = ex2(x[D] - finite(ms.x));
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    if (row < row0 + n) {
+      for (int i0 = run + part; i0 <= last; i0 += kEach * each) {
+        float y[kEach][D / 32];
+        float2 ml[kEach];
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] += f * x[32 * e + lane];
+        for (int k = 0; k < kEach; ++k) {
+          const int i = min(i0 + k * each, last);
+          const float* x = a.part + (((int64_t)i * 2 + (i == run ? 1 : 0)) * a.rows + row) * (D + kPad);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) y[k][e] = x[32 * e + lane];
+          ml[k] = *reinterpret_cast<const float2*>(x + D);
+          if (i0 + k * each > last) ml[k] = make_float2(-INFINITY, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          if (i0 + k * each > last) break;
+          const float up = fmaxf(top, ml[k].x);
+          const float f = ex2(top - finite(up)), w = ex2(ml[k].x - finite(up));
+          sum = sum * f + ml[k].y * w;
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) acc[e] = acc[e] * f + y[k][e] * w;
+          top = up;
+        }
+      }
     }
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) s_o[warp][32 * e + lane] = acc[e];
+    if (lane == 0) s_ml[warp][0] = top, s_ml[warp][1] = sum;
     __syncthreads();
-    for (int d = tid; d < D; d += kJoinThreads) {
+    for (int i = tid; i < n * D; i += kJoinThreads) {
+      const int r = i / D, d = i % D, j = h * a.groups + r0 + row0 + r;
+      top = -INFINITY;
+      for (int w = r * each; w < (r + 1) * each; ++w) top = fmaxf(top, s_ml[w][0]);
+      sum = 0.f;
       float y = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) y += s_o[w][d];
-      store_out(a, F16, to + d, y * inv);
-    }
-    if (tid == 0) a.lse[id] = (finite(ms.x) - a.offset + log2f(ms.y)) * 0.6931471805599453f;
-    return;
-  }
-  id -= (int64_t)a.batch * heads;
-  const int slice = (int)(id % slices), h = (int)(id / slices % a.kv), b = (int)(id / slices / a.kv);
-  const Span s(a, b);
-  const int t0 = slice * (kSlice / kUnit), t1 = min(t0 + kSlice / kUnit, s.units);
-  if (t0 >= t1) return;
-  const int64_t base = a.base[b];
-  for (int r = warp; r < a.groups; r += kWarps) {
-    const Pieces pc(a, base, s.units, h * a.rt + r / a.rows, total, active);
-    float lse2;
-    if (pc.first == pc.last) {
-      lse2 = a.lse2[(int64_t)b * heads + h * a.groups + r];
-    } else {
-      const float2 ms = join_row(a, pc, r % a.rows, lane);
-      lse2 = finite(ms.x) - a.offset + log2f(ms.y);
-    }
-    if (lane == 0) s_lse[r] = lse2;
-  }
-  __syncthreads();
-  for (int i = tid; i < (t1 - t0) * kUnit; i += kJoinThreads) {
-    const int t = t0 + i / kUnit, e = s.entry(t) + i % kUnit;
-    if (e >= s.n) continue;
-    const int page = paged::page_of(a.table + b * a.table_stride, e, a.log_page, a.pages);
-    if (page < 0) continue;
-    float sum = 0.f;
-    for (int rt = 0; rt < a.rt; ++rt) {
-      const int64_t u = base * (a.kv * a.rt) + (int64_t)(h * a.rt + rt) * s.units + t;
-      const float* x = a.scores + (u * kUnit + i % kUnit) * a.score_stride;
-      const int rows = min(a.rows, a.groups - rt * a.rows);
-      for (int r = 0; r < rows; ++r) {
-        const float lse2 = s_lse[rt * a.rows + r];
-        sum += lse2 == -INFINITY ? 0.f : ex2(x[r] - lse2);
+      for (int w = r * each; w < (r + 1) * each; ++w) {
+        const float f = ex2(s_ml[w][0] - finite(top));
+        sum += s_ml[w][1] * f;
+        y += s_o[w][d] * f;
+      }
+      store_out<F16>(a, b * a.out_sb + j * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
+      if (d == 0) {
+        const float lse2 = finite(top) - a.offset + log2f(sum);
+        a.lse[(int64_t)b * a.kv * a.groups + j] = lse2 * kLn2;
+        a.lse2[(int64_t)b * a.kv * a.groups + j] = lse2;
       }
     }
-    a.mass[page * a.meta_page + h * a.meta_head + (e & (a.page - 1))] += sum;
+    __syncthreads();
   }
+}
+
+// Adds the weights to the mass, from the scores in the workspace: a block takes 4 kMassThreads
+// entries of one (sequence, key head), a thread four of them.
+__global__ void __launch_bounds__(kMassThreads, 6)
+    paged_mass_kernel(const AttendArgs a) {
+  __shared__ float s_lse[64];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, h = blockIdx.x % a.kv, b = blockIdx.x / a.kv;
+  const Span s(a, b);
+  if (blockIdx.y * kMassThreads >= 4 * s.units) return;
+  const int64_t unit = a.base[b] * (a.kv * a.rt) + (int64_t)h * a.rt * s.units;
+  if (tid < a.groups) {
+    const float x = a.lse2[((int64_t)b * a.kv + h) * a.groups + tid];
+    s_lse[tid] = x == -INFINITY ? INFINITY : x;
+  }
+  __syncthreads();
+  for (int i = blockIdx.y * kMassThreads + tid; i < 4 * s.units; i += gridDim.y * kMassThreads)
+    add_weights(a, b, h, s, i, a.scores + unit * (kUnit * a.rows), (int64_t)s.units * (kUnit * a.rows), s_lse);
 }
 
 constexpr size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // What a launch needs beside the caller's arguments: row tiles, grid, workspace layout.
 struct Plan {
-  int groups, rt, rows, nt, warps_per_cta, ctas, score_stride, slices;
-  size_t base, part, lse2, scores, bytes;
+  int groups, rt, rows, nt, ctas, runs;
+  bool whole;
+  int64_t units_per_head;
+  size_t base, open, part, lse2, scores, bytes;
 };
 
 int sm_count() {
@@ -611,13 +735,19 @@ int sm_count() {
   return cached[dev] > 0 ? cached[dev] : 148;
 }
 
+// One CTA per key head (a single launch, no workspace without weights) while the heads fit the
+// SMs at once and a warp of the CTA walks few units; past that the equal runs win.
+bool whole_heads(int64_t heads, int64_t units_per_head, int row_tiles, int sms) {
+  return row_tiles == 1 && heads <= sms && units_per_head <= kWholeUnits;
+}
+
 Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_attend_desc& d) {
   Plan p;
   p.groups = d.h / c.kv;
   p.rt = (p.groups + 15) / 16;
   p.rows = (p.groups + p.rt - 1) / p.rt;
   p.nt = p.rows <= 8 ? 1 : 2;
-  p.warps_per_cta = c.d == 256 ? 4 : 8;
+  const int warps = c.d == 256 ? Shape<256>::kWarps : Shape<128>::kWarps;
   // the most units that the table allows
   const int64_t cap = (int64_t)b.width * c.page;
   int64_t per = (cap + kUnit - 1) / kUnit;
@@ -625,39 +755,66 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
     const int64_t bound = ((int64_t)d.sinks + kUnit - 1) / kUnit + ((int64_t)d.window + kUnit - 1) / kUnit + 1;
     if (bound < per) per = bound;
   }
-  const int64_t units = per * b.batch * c.kv * p.rt;
+  p.units_per_head = per;
+  const int64_t heads = (int64_t)b.batch * c.kv, units = per * heads * p.rt;
   const int sms = sm_count();
-  // short work is spread over all SMs, one warp each, before a second warp of an SM gets any
-  const int64_t spread = (units + kMinUnits - 1) / kMinUnits;
-  p.ctas = (int)(spread < 1 ? 1 : spread < sms ? spread : sms);
-  p.score_stride = (p.rows + 1) / 2 * 2;
-  p.slices = (int)((per * kUnit + kSlice - 1) / kSlice);
+  p.whole = whole_heads(heads, per, p.rt, sms);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += align256(bytes);
     return here;
   };
-  p.base = take(((size_t)b.batch + 1) * 8);
-  p.part = take((size_t)p.ctas * p.warps_per_cta * 2 * p.rows * (c.d + 2) * 4);
-  p.lse2 = take((size_t)b.batch * d.h * 4);
-  p.scores = d.accumulate ? take((size_t)units * kUnit * p.score_stride * 4) : 0;
+  p.base = p.open = p.part = p.lse2 = p.scores = 0;
+  if (p.whole) {
+    p.ctas = (int)heads, p.runs = 0;
+  } else {
+    // short work is spread over all SMs, one warp each, before a second warp of an SM gets any
+    const int64_t spread = (units + kMinUnits - 1) / kMinUnits;
+    p.ctas = (int)(spread < 1 ? 1 : spread < sms ? spread : sms);
+    p.runs = p.ctas * warps;
+    p.base = take(((size_t)b.batch + 1) * 8);
+    p.open = take((size_t)p.runs * 16);
+    p.part = take((size_t)p.runs * 2 * p.rows * (c.d + kPad) * 4);
+    p.lse2 = take((size_t)b.batch * d.h * 4);
+  }
+  if (d.accumulate) p.scores = take((size_t)units * kUnit * p.rows * 4);
   p.bytes = at;
   return p;
 }
 
+// The dynamic shared memory limit of a kernel, set once per device (bit dev of `done`).
+cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return e;
+}
+
+template <int D, int NT, bool F16, bool WHOLE>
+cudaError_t launch_kernel(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, const CUtensorMap& mv,
+                          cudaStream_t st) {
+  constexpr int smem = kRing + 1024;
+  static std::atomic<uint64_t> done{0};
+  auto* kernel = paged_attend_kernel<D, NT, F16, WHOLE>;
+  const cudaError_t e = allow_smem((const void*)kernel, smem, done);
+  if (e != cudaSuccess) return e;
+  kernel<<<p.ctas, 32 * Shape<D>::kWarps, smem, st>>>(mk, mv, a);
+  return cudaGetLastError();
+}
+
 template <int D, int NT, bool F16>
 cudaError_t launch(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  using S = Shape<D>;
-  constexpr int smem = kRing + 1024;
-  auto* kernel = paged_attend_kernel<D, NT, F16>;
-  cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (p.whole) return launch_kernel<D, NT, F16, true>(a, p, mk, mv, st);
+  const cudaError_t e = launch_kernel<D, NT, F16, false>(a, p, mk, mv, st);
   if (e != cudaSuccess) return e;
-  kernel<<<p.ctas, 32 * S::kWarps, smem, st>>>(mk, mv, a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  const int64_t blocks = (int64_t)a.batch * a.kv * a.groups + (a.accumulate ? (int64_t)a.batch * a.kv * p.slices : 0);
-  cfg.gridDim = dim3((unsigned)blocks);
+  const int64_t query_heads = (int64_t)a.batch * a.kv * a.groups;
+  const bool by_head = query_heads <= p.runs;
+  cfg.gridDim = dim3((unsigned)(by_head ? query_heads : p.runs));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -665,7 +822,12 @@ cudaError_t launch(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, co
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, F16>, a, p.ctas * S::kWarps, p.slices);
+  const cudaError_t j = cudaLaunchKernelEx(&cfg, paged_join_kernel<D, F16>, a, p.runs, by_head);
+  if (j != cudaSuccess || !a.accumulate) return j;
+  const int64_t slices = (p.units_per_head * 4 + kMassThreads - 1) / kMassThreads;
+  cfg.gridDim = dim3((unsigned)((int64_t)a.batch * a.kv), (unsigned)(slices < 65535 ? slices : 65535));
+  cfg.blockDim = dim3(kMassThreads);
+  return cudaLaunchKernelEx(&cfg, paged_mass_kernel, a);
 }
 
 template <int D>
@@ -697,10 +859,11 @@ cudaError_t launch_paged_attend(const pbk_paged_cache& c, const pbk_paged_batch&
   a.mass = c.mass, a.meta_page = c.meta_page, a.meta_head = c.meta_head, a.pages = c.pages;
   uint8_t* w = static_cast<uint8_t*>(ws);
   a.base = reinterpret_cast<int64_t*>(w + p.base);
+  a.open = reinterpret_cast<int4*>(w + p.open);
   a.part = reinterpret_cast<float*>(w + p.part);
   a.lse2 = reinterpret_cast<float*>(w + p.lse2);
   a.scores = reinterpret_cast<float*>(w + p.scores);
-  a.score_stride = p.score_stride, a.d = c.d;
+  a.whole_units = p.units_per_head;
   a.err = device_error_word();
   CUtensorMap mk, mv;
   {

@@ -92,7 +92,7 @@ class PagedCache:
             d.meta_page, d.meta_head = t.stride()[:2]
         d.mass = None if self.mass is None else self.mass.data_ptr()
         d.pos = None if self.pos is None else self.pos.data_ptr()
-        self._ref = _byref(d)
+        self._ref, self._index = _byref(d), self.device.index
 
     @classmethod
     def allocate(cls, pages: int, kv: int, page: int, hd: int, dtype: torch.dtype = torch.bfloat16,
@@ -112,32 +112,26 @@ class PagedCache:
         return self._desc.page
 
 
-class _on:
-    """The device of a cache as the current one (nothing to do when it already is)."""
-    __slots__ = ("dev", "prev")
-
-    def __init__(self, dev: torch.device):
-        self.dev = dev.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
-        return False
+def _call(cache: PagedCache, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the cache's device and its current stream; raises on an error. A
+    serving step makes many small calls, so the common case (that device is current) takes the
+    stream's handle without making a Stream object."""
+    i = cache._index
+    if torch.cuda.current_device() == i:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(i)), what)
+    else:
+        with torch.cuda.device(i):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(i)), what)
 
 
 def _batch(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor | None, seen: torch.Tensor | None = None):
-    dev = cache.device
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != dev or table.stride(1) != 1:
+    i = cache._index
+    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != i or table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, M] on the cache's GPU with contiguous rows")
     b, m = table.shape
     for t, name in ((lengths, "lengths"), (seen, "seen")):
-        if t is not None and (t.dtype != torch.int32 or t.device != dev or t.shape != (b,) or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != b or t.get_device() != i
+                              or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous int32 [{b}] on the cache's GPU")
     return PbkPagedBatch(b, m, table.data_ptr(), table.stride(0), None if lengths is None else lengths.data_ptr(),
                          None if seen is None else seen.data_ptr())
@@ -151,13 +145,18 @@ def _need(cache: PagedCache, what: str, *names: str) -> None:
 
 def _rows(t: torch.Tensor, cache: PagedCache, what: str) -> None:
     k = cache.k_pages
-    if t.device != cache.device or t.dtype != k.dtype or t.shape[-1] != k.shape[3] or t.stride(-1) != 1:
+    if t.get_device() != cache._index or t.dtype != k.dtype or t.size(-1) != cache._desc.d or t.stride(-1) != 1:
         raise ValueError(f"{what}: {k.dtype} with a contiguous last dim of {k.shape[3]} on the cache's GPU expected, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _run(cache: PagedCache, fn, what: str, nbytes: int, *args) -> None:
+    """_call with a workspace of nbytes from the caching allocator behind the other arguments."""
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
+        _call(cache, fn, what, *args, ws.data_ptr(), nbytes)
+    else:
+        _call(cache, fn, what, *args, None, 0)
 
 
 def paged_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -180,10 +179,8 @@ def paged_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_tab
             raise ValueError(f"cu_seqlens must be contiguous int32 [{b.batch + 1}] on the cache's GPU")
     elif k.shape[0] != b.batch:
         raise ValueError(f"paged_append_: {k.shape[0]} tokens for {b.batch} sequences need cu_seqlens")
-    with _on(cache.device) as stream:
-        check(LIB.pbk_paged_append(cache._ref, _byref(b), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
-                                   k.shape[0], None if cu_seqlens is None else cu_seqlens.data_ptr(), stream),
-              "pbk_paged_append")
+    _call(cache, LIB.pbk_paged_append, "pbk_paged_append", cache._ref, _byref(b), k.data_ptr(), v.data_ptr(),
+          k.stride(0), k.stride(1), k.size(0), None if cu_seqlens is None else cu_seqlens.data_ptr())
 
 
 def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -205,7 +202,7 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
         raise ValueError("paged_attend: the window holds at least the new token (None: no window)")
     n, h, d = q.shape
     if out is None:
-        out = torch.empty(n, h, d, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype not in (q.dtype, torch.float32) or out.stride(-1) != 1 \
             or out.device != q.device:
         raise ValueError(f"paged_attend: out must be {tuple(q.shape)}, {q.dtype} or fp32, with a contiguous last dim")
@@ -214,10 +211,8 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
                               _DTYPES[out.dtype], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
                               out.stride(1), lse.data_ptr())
     bref, dref = _byref(b), _byref(desc)
-    with _on(cache.device) as stream:
-        ws = _workspace(LIB.pbk_paged_attend_workspace(cache._ref, bref, dref), q.device)
-        check(LIB.pbk_paged_attend(cache._ref, bref, dref, None if ws is None else ws.data_ptr(),
-                                   0 if ws is None else ws.numel(), stream), "pbk_paged_attend")
+    _run(cache, LIB.pbk_paged_attend, "pbk_paged_attend", LIB.pbk_paged_attend_workspace(cache._ref, bref, dref),
+         cache._ref, bref, dref)
     return out, lse
 
 
@@ -236,10 +231,8 @@ def paged_observe_(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor
     desc = PbkPagedObserveDesc(q.shape[2], q.shape[1], q.shape[3] ** -0.5 if scale is None else scale, 0, q.data_ptr(),
                                q.stride(0), q.stride(1), q.stride(2))
     bref, dref = _byref(b), _byref(desc)
-    with _on(cache.device) as stream:
-        ws = _workspace(LIB.pbk_paged_observe_workspace(cache._ref, bref, dref), q.device)
-        check(LIB.pbk_paged_observe(cache._ref, bref, dref, None if ws is None else ws.data_ptr(),
-                                    0 if ws is None else ws.numel(), stream), "pbk_paged_observe")
+    _run(cache, LIB.pbk_paged_observe, "pbk_paged_observe", LIB.pbk_paged_observe_workspace(cache._ref, bref, dref),
+         cache._ref, bref, dref)
 
 
 def select_evictions(cache: PagedCache, block_table: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor,
@@ -259,11 +252,8 @@ def select_evictions(cache: PagedCache, block_table: torch.Tensor, lengths: torc
     src, dst = places.unbind(0)
     count = torch.empty(b.batch, cache.kv, dtype=torch.int32, device=cache.device)
     bref = _byref(b)
-    with _on(cache.device) as stream:
-        ws = _workspace(LIB.pbk_paged_select_workspace(cache._ref, bref, budget), cache.device)
-        check(LIB.pbk_paged_select(cache._ref, bref, budget, recent, sinks, src.data_ptr(), dst.data_ptr(),
-                                   count.data_ptr(), moves, None if ws is None else ws.data_ptr(),
-                                   0 if ws is None else ws.numel(), stream), "pbk_paged_select")
+    _run(cache, LIB.pbk_paged_select, "pbk_paged_select", LIB.pbk_paged_select_workspace(cache._ref, bref, budget),
+         cache._ref, bref, budget, recent, sinks, src.data_ptr(), dst.data_ptr(), count.data_ptr(), moves)
     return src, dst, count
 
 
@@ -278,9 +268,8 @@ def move_entries_(cache: PagedCache, block_table: torch.Tensor, src: torch.Tenso
     for t, name in ((src, "src"), (dst, "dst"), (count, "count")):
         if t.dtype != torch.int32 or not t.is_contiguous() or t.device != cache.device:
             raise ValueError(f"move_entries_: {name} must be contiguous int32 on the cache's GPU")
-    with _on(cache.device) as stream:
-        check(LIB.pbk_paged_move(cache._ref, _byref(b), src.data_ptr(), dst.data_ptr(), count.data_ptr(), src.shape[2],
-                                 stream), "pbk_paged_move")
+    _call(cache, LIB.pbk_paged_move, "pbk_paged_move", cache._ref, _byref(b), src.data_ptr(), dst.data_ptr(),
+          count.data_ptr(), src.size(2))
 
 
 def paged_evict_(cache: PagedCache, block_table: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor, budget: int,
