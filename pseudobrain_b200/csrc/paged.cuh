@@ -27,7 +27,26 @@ __device__ __forceinline__ int page_of(const int32_t* row, int j, int log_page, 
   return (unsigned)id < (unsigned)pages ? id : -1;
 }
 
+// The cache's kernels are launched so that each may start while the one before it in the stream
+// ends (programmatic dependent launch): every kernel lets its successor start at once and waits
+// for its predecessor's writes before it touches memory. A serving step is a chain of short
+// kernels, and this hides most of each launch.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace paged
+
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = (size_t)smem, cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
 #endif
 
 inline int paged_log2(int x) {

@@ -9,6 +9,8 @@ namespace {
 __global__ void __launch_bounds__(256)
     paged_append_kernel(const pbk_paged_cache c, const pbk_paged_batch b, const uint16_t* k, const uint16_t* v,
                         int64_t stride_t, int64_t stride_h, int tokens, const int32_t* cu, int log_page) {
+  paged::launch_next();
+  paged::wait_previous();
   const int chunks = c.d >> 3;
   const int64_t work = (int64_t)tokens * c.kv * chunks;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < work; i += (int64_t)gridDim.x * blockDim.x) {
@@ -47,6 +49,8 @@ __global__ void __launch_bounds__(256)
 __global__ void __launch_bounds__(256)
     paged_move_kernel(const pbk_paged_cache c, const pbk_paged_batch b, const int32_t* src, const int32_t* dst,
                       const int32_t* count, int moves, int log_page) {
+  paged::launch_next();
+  paged::wait_previous();
   const int h = blockIdx.y, s = blockIdx.z;
   const int64_t row = (int64_t)s * c.kv + h;
   const int n = min(count[row], moves);
@@ -89,6 +93,8 @@ constexpr int kSelThreads = 1024;
 __global__ void __launch_bounds__(kSelThreads)
     paged_select_kernel(const pbk_paged_cache c, const pbk_paged_batch b, int budget, int recent, int sinks,
                         int32_t* src, int32_t* dst, int32_t* count, int moves, int log_page) {
+  paged::launch_next();
+  paged::wait_previous();
   const int h = blockIdx.x, s = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t orow = (int64_t)s * c.kv + h;
@@ -181,27 +187,24 @@ cudaError_t launch_paged_append(const pbk_paged_cache& c, const pbk_paged_batch&
                                 cudaStream_t st) {
   const int64_t work = (int64_t)tokens * c.kv * (c.d / 8);
   const int64_t blocks = (work + 255) / 256;
-  paged_append_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(
-      c, b, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_t, stride_h, tokens, cu_seqlens,
-      paged_log2(c.page));
-  return cudaGetLastError();
+  return launch_after(paged_append_kernel, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, c, b,
+                      static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_t, stride_h, tokens,
+                      cu_seqlens, paged_log2(c.page));
 }
 
 size_t paged_select_workspace(const pbk_paged_cache&, const pbk_paged_batch&, int) { return 0; }
 
 cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
                                 int32_t* src, int32_t* dst, int32_t* count, int moves, void*, cudaStream_t st) {
-  paged_select_kernel<<<dim3(c.kv, b.batch), kSelThreads, 0, st>>>(c, b, budget, recent, sinks, src, dst, count, moves,
-                                                                  paged_log2(c.page));
-  return cudaGetLastError();
+  return launch_after(paged_select_kernel, dim3(c.kv, b.batch), dim3(kSelThreads), 0, st, c, b, budget, recent, sinks, src,
+                      dst, count, moves, paged_log2(c.page));
 }
 
 cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
                               const int32_t* dst, const int32_t* count, int moves, cudaStream_t st) {
   const int64_t blocks = ((int64_t)moves * (c.d / 8) + 255) / 256;
-  paged_move_kernel<<<dim3((unsigned)(blocks < 64 ? blocks : 64), c.kv, b.batch), 256, 0, st>>>(c, b, src, dst, count, moves,
-                                                                                            paged_log2(c.page));
-  return cudaGetLastError();
+  return launch_after(paged_move_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), c.kv, b.batch), dim3(256), 0, st, c, b, src,
+                      dst, count, moves, paged_log2(c.page));
 }
 
 }  // namespace pbk

@@ -97,10 +97,11 @@ class PagedCache:
     @classmethod
     def allocate(cls, pages: int, kv: int, page: int, hd: int, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str = "cuda", weights: bool = True) -> "PagedCache":
-        """A pool of ``pages`` pages; with ``weights`` also mass and pos (for eviction)."""
+        """A pool of ``pages`` pages (keys and values uninitialised); with ``weights`` also mass and
+        pos, zeroed (for eviction)."""
         k = torch.empty(pages, kv, page, hd, dtype=dtype, device=device)
-        mass = torch.empty(pages, kv, page, dtype=torch.float32, device=device) if weights else None
-        pos = torch.empty(pages, kv, page, dtype=torch.int32, device=device) if weights else None
+        mass = torch.zeros(pages, kv, page, dtype=torch.float32, device=device) if weights else None
+        pos = torch.zeros(pages, kv, page, dtype=torch.int32, device=device) if weights else None
         return cls(k, torch.empty_like(k), mass, pos)
 
     @property
