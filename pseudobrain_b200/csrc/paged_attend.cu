@@ -7,9 +7,9 @@
 // walks its run with an online softmax (base 2) and writes a head's result when its run holds
 // the whole head, else the partial (maximum, sum, weighted values) of its piece; the join
 // kernel, launched behind it, merges the pieces of each head and, when asked, turns the scores
-// kept in the workspace into weights and adds them to the cache's mass. Few short heads take
-// the other way: one CTA per head, whose warps share its units and join in shared memory, one
-// launch in all (see `whole_heads`).
+// kept in the workspace into weights and adds them to the cache's mass. Few heads of moderate
+// length take the other way: a cluster of 1 to 8 CTAs per head, whose warps share its units and
+// join through distributed shared memory, one launch in all (see `head_cluster`).
 #include <atomic>
 
 #include "common.cuh"
@@ -23,7 +23,7 @@ namespace {
 constexpr int kUnit = 16;           // entries per unit
 constexpr int kRing = 192 * 1024;   // staging bytes per CTA
 constexpr int kMinUnits = 2;        // units per warp below which fewer warps take part
-constexpr int kWholeUnits = 128;    // most units per head where one CTA takes a whole head
+constexpr int kClusterUnits = 160;  // most units per CTA where a cluster takes a whole head
 constexpr int kJoinThreads = 256;
 constexpr int kMassThreads = 256;
 constexpr int kPad = 4;             // floats after a partial row's D values: maximum, sum, two unused
@@ -208,6 +208,28 @@ __device__ __forceinline__ void add_weights(const AttendArgs& a, int b, int h, c
   }
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t x;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(x));
+  return x;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t x;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(x));
+  return x;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float of CTA `rank`'s shared memory, at the place that `p` has in this CTA's.
+__device__ __forceinline__ float remote(const float* p, uint32_t rank) {
+  uint32_t at;
+  float x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+
 // Keys are the M of both products and the query rows their N: S^T = K Q^T (A = 16 keys by
 // ldmatrix, B = Q^T in registers) and O^T += V^T P^T (A = V^T by ldmatrix.trans, B = P^T from
 // S^T's accumulators by two 8 x 8 transposes). With at most 16 rows the tcgen05 shapes would
@@ -235,9 +257,12 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   __shared__ uint64_t s_full[S::kWarps][S::kStages];
   __shared__ int64_t s_sum[S::kWarps], s_off[S::kWarps];
   __shared__ int s_seq[S::kWarps];
+  __shared__ float2 s_ml[WHOLE ? S::kWarps : 1][16], s_joined[16];  // WHOLE: (maximum, sum) per row
+  __shared__ float s_lse[16];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nwarps = gridDim.x * S::kWarps;
   const int pairs = a.kv * a.rt;  // (key head, row tile) of a sequence
+  const uint32_t rank = WHOLE ? cluster_rank() : 0, ctas = WHOLE ? cluster_size() : 1;
   paged::launch_next();
   if (tid == 0) {
     tc::prefetch_tmap(&mk);
@@ -259,12 +284,13 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   int64_t u0 = 0;  // the run's first unit in the line (WHOLE: among the scores set apart)
   int run = 0, length = 0, count;
   if (WHOLE) {
-    c.b = blockIdx.x / pairs;
-    c.pair = blockIdx.x % pairs;
+    const int head = blockIdx.x / ctas, part = rank * S::kWarps + warp, parts = ctas * S::kWarps;
+    c.b = head / pairs;
+    c.pair = head % pairs;
     c.s = Span(a, c.b);
-    c.t = c.s.units * warp / S::kWarps;
-    count = c.s.units * (warp + 1) / S::kWarps - c.t;
-    u0 = blockIdx.x * a.whole_units + c.t;
+    c.t = (int)((int64_t)c.s.units * part / parts);
+    count = (int)((int64_t)c.s.units * (part + 1) / parts) - c.t;
+    u0 = head * a.whole_units + c.t;
   } else {
     // ---- where each warp's run starts: a scan of the sequences' units by the whole CTA
     const int per = (a.batch + kThreads - 1) / kThreads;
@@ -561,49 +587,67 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     for (int s = 0; s < S::kStages; ++s) tc::mbar_wait(&s_full[warp][s], parity, 200000000ull);
   if (!WHOLE) return;
 
-  // ---- WHOLE: the warps' parts, each in its own (now free) ring, joined by the CTA
+  // ---- WHOLE: the warps' parts, each in its own (now free) ring, joined by the CTA into the
+  // first warp's, and the CTAs' by the cluster
   float* mine = reinterpret_cast<float*>(my_ring);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float sum = column_sum(l[nt][r]);
-      float* to = mine + (8 * nt + 2 * t4 + r) * (D + kPad);
+      const int row = 8 * nt + 2 * t4 + r;
 #pragma unroll
       for (int kk = 0; kk < kK; ++kk) {
-        to[16 * kk + g] = o[nt][kk][r];
-        to[16 * kk + 8 + g] = o[nt][kk][2 + r];
+        mine[row * D + 16 * kk + g] = o[nt][kk][r];
+        mine[row * D + 16 * kk + 8 + g] = o[nt][kk][2 + r];
       }
-      if (g == 0) to[D] = m[nt][r], to[D + 1] = sum;
+      if (g == 0) s_ml[warp][row] = make_float2(m[nt][r], sum);
     }
   __syncthreads();
-  __shared__ float s_lse[16];
-  const int h = c.pair;
-  auto part = [&](int w, int row) {
-    return reinterpret_cast<const float*>(ring + w * S::kStages * 2 * S::kTile) + row * (D + kPad);
-  };
+  float* joined = reinterpret_cast<float*>(ring);
   for (int i = tid; i < rows * D; i += kThreads) {
-    const int row = i / D, d = i % D, j = h * a.groups + row;
-    float top = -INFINITY, sum = 0.f, y = 0.f;
+    float top = -INFINITY, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, part(w, row)[D]);
+    for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, s_ml[w][i / D].x);
 #pragma unroll
-    for (int w = 0; w < S::kWarps; ++w) {
-      const float f = ex2(part(w, row)[D] - finite(top));
-      sum += part(w, row)[D + 1] * f;
-      y += part(w, row)[d] * f;
-    }
-    store_out<F16>(a, c.b * a.out_sb + j * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
-    if (d == 0) {
-      const float lse2 = finite(top) - a.offset + log2f(sum);
-      a.lse[(int64_t)c.b * a.kv * a.groups + j] = lse2 * kLn2;
-      s_lse[row] = lse2 == -INFINITY ? INFINITY : lse2;  // a row without weight adds 0
-    }
+    for (int w = 0; w < S::kWarps; ++w)
+      y += reinterpret_cast<const float*>(ring + w * S::kStages * 2 * S::kTile)[i] * ex2(s_ml[w][i / D].x - finite(top));
+    joined[i] = y;  // read and written by this thread only
   }
+  if (tid < rows) {
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, s_ml[w][tid].x);
+    for (int w = 0; w < S::kWarps; ++w) sum += s_ml[w][tid].y * ex2(s_ml[w][tid].x - finite(top));
+    s_joined[tid] = make_float2(top, sum);
+  }
+  cluster_sync();
+  const int h = c.pair;
+  for (int i = rank * kThreads + tid; i < rows * D; i += ctas * kThreads) {
+    const int row = i / D, d = i % D;
+    float top = -INFINITY, sum = 0.f, y = 0.f;
+    for (uint32_t k = 0; k < ctas; ++k) top = fmaxf(top, remote(&s_joined[row].x, k));
+    for (uint32_t k = 0; k < ctas; ++k) {
+      const float f = ex2(remote(&s_joined[row].x, k) - finite(top));
+      sum += remote(&s_joined[row].y, k) * f;
+      y += remote(&joined[i], k) * f;
+    }
+    store_out<F16>(a, c.b * a.out_sb + (h * a.groups + row) * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
+  }
+  if (tid < rows) {
+    float top = -INFINITY, sum = 0.f;
+    for (uint32_t k = 0; k < ctas; ++k) top = fmaxf(top, remote(&s_joined[tid].x, k));
+    for (uint32_t k = 0; k < ctas; ++k) sum += remote(&s_joined[tid].y, k) * ex2(remote(&s_joined[tid].x, k) - finite(top));
+    const float lse2 = finite(top) - a.offset + log2f(sum);
+    if (rank == 0) a.lse[(int64_t)c.b * a.kv * a.groups + h * a.groups + tid] = lse2 * kLn2;
+    s_lse[tid] = lse2 == -INFINITY ? INFINITY : lse2;  // a row without weight adds 0
+  }
+  cluster_sync();  // no CTA leaves while another reads its part
   if (!a.accumulate) return;
-  __syncthreads();
-  for (int i = tid; i < 4 * c.s.units; i += kThreads)
-    add_weights(a, c.b, h, c.s, i, a.scores + blockIdx.x * a.whole_units * (kUnit * a.rows), 0, s_lse);
+  // this CTA's warps wrote the scores of its own units
+  const int t0 = (int)((int64_t)c.s.units * (rank * S::kWarps) / (ctas * S::kWarps));
+  const int t1 = (int)((int64_t)c.s.units * ((rank + 1) * S::kWarps) / (ctas * S::kWarps));
+  for (int i = 4 * t0 + tid; i < 4 * t1; i += kThreads)
+    add_weights(a, c.b, h, c.s, i, a.scores + (blockIdx.x / ctas) * a.whole_units * (kUnit * a.rows), 0, s_lse);
 }
 
 // Joins the heads that no run held whole: the warps of a block share a head's rows and each
@@ -732,8 +776,7 @@ constexpr size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
 // What a launch needs beside the caller's arguments: row tiles, grid, workspace layout.
 struct Plan {
-  int groups, rt, rows, nt, ctas, runs;
-  bool whole;
+  int groups, rt, rows, nt, ctas, runs, cluster;
   int64_t units_per_head;
   size_t base, open, part, lse2, scores, bytes;
 };
@@ -746,10 +789,17 @@ int sm_count() {
   return cached[dev] > 0 ? cached[dev] : 148;
 }
 
-// One CTA per key head (a single launch, no workspace without weights) while the heads fit the
-// SMs at once and a warp of the CTA walks few units; past that the equal runs win.
-bool whole_heads(int64_t heads, int64_t units_per_head, int row_tiles, int sms) {
-  return row_tiles == 1 && heads <= sms && units_per_head <= kWholeUnits;
+// CTAs per key head where a cluster takes a whole head (one launch, no workspace without
+// weights), 0 where the equal runs and their join are better. The join costs about 6 us at any
+// size; a cluster costs SMs that its size leaves over and, with ragged lengths, the time of the
+// longest sequence, so it is for heads that fit the SMs at once and CTAs that walk at most
+// kClusterUnits units, by the table's capacity. Clusters of more than one CTA are packed by GPC,
+// which leaves an eighth of the SMs over.
+int head_cluster(int64_t heads, int64_t units_per_head, int row_tiles, int sms) {
+  if (row_tiles > 1 || heads > sms) return 0;
+  int c = 1;
+  while (c < 8 && units_per_head > 2 * Shape<128>::kWarps * c && heads * 2 * c <= sms - sms / 8) c *= 2;
+  return units_per_head <= (int64_t)kClusterUnits * c ? c : 0;
 }
 
 Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_attend_desc& d) {
@@ -769,7 +819,7 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
   p.units_per_head = per;
   const int64_t heads = (int64_t)b.batch * c.kv, units = per * heads * p.rt;
   const int sms = sm_count();
-  p.whole = whole_heads(heads, per, p.rt, sms);
+  p.cluster = head_cluster(heads, per, p.rt, sms);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -777,8 +827,8 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
     return here;
   };
   p.base = p.open = p.part = p.lse2 = p.scores = 0;
-  if (p.whole) {
-    p.ctas = (int)heads, p.runs = 0;
+  if (p.cluster > 0) {
+    p.ctas = (int)heads * p.cluster, p.runs = 0;
   } else {
     // short work is spread over all SMs, one warp each, before a second warp of an SM gets any
     const int64_t spread = (units + kMinUnits - 1) / kMinUnits;
@@ -813,23 +863,23 @@ cudaError_t launch_kernel(const AttendArgs& a, const Plan& p, const CUtensorMap&
   auto* kernel = paged_attend_kernel<D, NT, F16, WHOLE>;
   const cudaError_t e = allow_smem((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
-  return launch_after(kernel, dim3((unsigned)p.ctas), dim3(32 * Shape<D>::kWarps), smem, st, mk, mv, a);
+  return launch_after(kernel, dim3((unsigned)p.ctas), dim3(32 * Shape<D>::kWarps), smem, st, WHOLE ? p.cluster : 1, mk, mv, a);
 }
 
 template <int D, int NT, bool F16>
 cudaError_t launch(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
-  if (p.whole) return launch_kernel<D, NT, F16, true>(a, p, mk, mv, st);
+  if (p.cluster > 0) return launch_kernel<D, NT, F16, true>(a, p, mk, mv, st);
   const cudaError_t e = launch_kernel<D, NT, F16, false>(a, p, mk, mv, st);
   if (e != cudaSuccess) return e;
   const int64_t query_heads = (int64_t)a.batch * a.kv * a.groups;
   const bool by_head = query_heads <= p.runs;
   const cudaError_t j = launch_after(paged_join_kernel<D, F16>, dim3((unsigned)(by_head ? query_heads : p.runs)),
-                                     dim3(kJoinThreads), 0, st, a, p.runs, by_head);
+                                     dim3(kJoinThreads), 0, st, 1, a, p.runs, by_head);
   if (j != cudaSuccess || !a.accumulate) return j;
   const int64_t slices = (p.units_per_head * 4 + kMassThreads - 1) / kMassThreads;
   return launch_after(paged_mass_kernel,
                       dim3((unsigned)((int64_t)a.batch * a.kv), (unsigned)(slices < 65535 ? slices : 65535)),
-                      dim3(kMassThreads), 0, st, a);
+                      dim3(kMassThreads), 0, st, 1, a);
 }
 
 template <int D>

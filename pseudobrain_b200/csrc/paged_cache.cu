@@ -187,7 +187,7 @@ cudaError_t launch_paged_append(const pbk_paged_cache& c, const pbk_paged_batch&
                                 cudaStream_t st) {
   const int64_t work = (int64_t)tokens * c.kv * (c.d / 8);
   const int64_t blocks = (work + 255) / 256;
-  return launch_after(paged_append_kernel, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, c, b,
+  return launch_after(paged_append_kernel, dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, 1, c, b,
                       static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), stride_t, stride_h, tokens,
                       cu_seqlens, paged_log2(c.page));
 }
@@ -196,14 +196,14 @@ size_t paged_select_workspace(const pbk_paged_cache&, const pbk_paged_batch&, in
 
 cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
                                 int32_t* src, int32_t* dst, int32_t* count, int moves, void*, cudaStream_t st) {
-  return launch_after(paged_select_kernel, dim3(c.kv, b.batch), dim3(kSelThreads), 0, st, c, b, budget, recent, sinks, src,
+  return launch_after(paged_select_kernel, dim3(c.kv, b.batch), dim3(kSelThreads), 0, st, 1, c, b, budget, recent, sinks, src,
                       dst, count, moves, paged_log2(c.page));
 }
 
 cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
                               const int32_t* dst, const int32_t* count, int moves, cudaStream_t st) {
   const int64_t blocks = ((int64_t)moves * (c.d / 8) + 255) / 256;
-  return launch_after(paged_move_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), c.kv, b.batch), dim3(256), 0, st, c, b, src,
+  return launch_after(paged_move_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), c.kv, b.batch), dim3(256), 0, st, 1, c, b, src,
                       dst, count, moves, paged_log2(c.page));
 }
 
