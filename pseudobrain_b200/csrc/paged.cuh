@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pbk.h"
 
 namespace pbk {
@@ -51,6 +53,28 @@ cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, int s
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 #endif
+
+// SMs of the current device (looked up once per device).
+inline int paged_sm_count() {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if ((n = cached[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// The dynamic shared memory limit of a kernel, set once per device (bit dev of `done`).
+inline cudaError_t paged_allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return e;
+}
 
 inline int paged_log2(int x) {
   int l = 0;

@@ -781,14 +781,6 @@ struct Plan {
   size_t base, open, part, lse2, scores, bytes;
 };
 
-int sm_count() {
-  static int cached[64] = {};
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (cached[dev] == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) cached[dev] = n;
-  return cached[dev] > 0 ? cached[dev] : 148;
-}
-
 // CTAs per key head where a cluster takes a whole head (one launch, no workspace without
 // weights), 0 where the equal runs and their join are better. The join costs about 6 us at any
 // size; a cluster costs SMs that its size leaves over and, with ragged lengths, the time of the
@@ -818,7 +810,7 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
   }
   p.units_per_head = per;
   const int64_t heads = (int64_t)b.batch * c.kv, units = per * heads * p.rt;
-  const int sms = sm_count();
+  const int sms = paged_sm_count();
   p.cluster = head_cluster(heads, per, p.rt, sms);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -844,24 +836,13 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
   return p;
 }
 
-// The dynamic shared memory limit of a kernel, set once per device (bit dev of `done`).
-cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
-  return e;
-}
-
 template <int D, int NT, bool F16, bool WHOLE>
 cudaError_t launch_kernel(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, const CUtensorMap& mv,
                           cudaStream_t st) {
   constexpr int smem = kRing + 1024;
   static std::atomic<uint64_t> done{0};
   auto* kernel = paged_attend_kernel<D, NT, F16, WHOLE>;
-  const cudaError_t e = allow_smem((const void*)kernel, smem, done);
+  const cudaError_t e = paged_allow_smem((const void*)kernel, smem, done);
   if (e != cudaSuccess) return e;
   return launch_after(kernel, dim3((unsigned)p.ctas), dim3(32 * Shape<D>::kWarps), smem, st, WHOLE ? p.cluster : 1, mk, mv, a);
 }

@@ -1,112 +1,508 @@
-// The attention weights of a prompt's last queries over the paged cache.
+// The attention weights of a prompt's last queries over the paged cache, summed into its mass.
+//
+// For every (sequence, key head) there are rows = queries x query heads of the key head, and
+// mass_j += sum_r 2^(s_rj - lse_r) with s = c q.k (c = scale log2 e) over the entries j that row r
+// sees. The rows' logarithms come first, so the scores are computed twice:
+//   pass 1: S = Q K^T   (tcgen05, M = 128 rows, N = 128 entries): a thread holds one row of the
+//           tile and keeps its running maximum and sum, no exchange between threads;
+//   pass 2: S^T = K Q^T (M = 128 entries, N = rows): a thread holds one entry and sums its
+//           weights over the rows, then adds them to the mass once. No atomics.
+// Storing the scores instead would cost 4 bytes per (row, entry), more than the keys themselves
+// from 64 rows of a head of 128 on.
+//
+// Keys are cut into tiles of 128 entries of one (sequence, key head); all tiles stand in one line
+// and each CTA (one per SM) takes an equal run of it. Row tiles hold as many whole queries as fit
+// 128 rows; up to kMaxTiles of them share each key tile, more take further launches. Warps: 0
+// TMA producer (keys page by page, queries as one box of heads x queries), 1 MMA issuer, 2-5 and
+// 6-9 two groups that take alternate key tiles from four accumulators in TMEM. Every wait is
+// bounded; on timeout the kernel records an error code and winds down.
+//
+// What bounds it: per key tile and pass 128 x 128 exponentials (16 a clock and SM: 0.55 us), the
+// keys' bytes (32 KB at an SM's share of HBM: 0.75 us) and 0.37 us of MMA.
+#include <atomic>
+
 #include "common.cuh"
 #include "paged.cuh"
+#include "tc.cuh"
+#include "tma_host.h"
 
 namespace pbk {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kTile = 128;       // entries of a key tile, rows of a row tile
+constexpr int kMaxTiles = 8;     // row tiles of a launch
+constexpr int kThreads = 320;
+constexpr int kGroup = 128;      // threads of an epilogue group
+constexpr uint32_t kTmemCols = 512;
 
-// A maximum over no scores (or over -inf alone) as 0: exp(-inf - 0) is then 0 without a branch,
-// and a NaN score stays NaN.
-__device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
+template <int D>
+struct Shape {
+  static constexpr int kBytes = kTile * D * 2;  // a tile of keys or queries
+  static constexpr int kBlock = kTile * 128;    // its 64-element columns: 128 rows of 128 bytes
+  static constexpr int kKeys = D == 64 ? 6 : D == 128 ? 3 : 2;
+  static constexpr int kQueries = D == 256 ? 1 : 2;
+  static constexpr int kSmem = (kKeys + kQueries) * kBytes + 1024;
+};
 
-template <bool F16>
-__device__ __forceinline__ float2 pair_f32(uint32_t x) {
-  if (F16) return __half22float2(*reinterpret_cast<const __half2*>(&x));
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
-}
-
-// One query row (a query head of one token) against the entries [0, end) of a sequence that
-// `visible` admits: lane l of a warp holds the dims 2l + 64 i, a warp takes every eighth entry.
-struct Rows {
-  const uint16_t* k;
-  const uint16_t* v;
+struct ObserveArgs {
   const int32_t* table;
-  int64_t sp, se, head;  // strides; the head's offset
-  int log_page, pages, pmask;
-  __device__ const uint16_t* at(const uint16_t* base, int j) const {
-    const int page = paged::page_of(table, j, log_page, pages);
-    return page < 0 ? nullptr : base + page * sp + head + (j & pmask) * se;
+  int64_t table_stride;
+  const int32_t* lengths;
+  int batch, width, page, log_page, pages;
+  int kv, groups, queries;       // key heads, query heads per key head, queries of the whole call
+  int w0, nw, tiles;             // first query of this launch, queries per row tile, row tiles
+  float c;                       // scale log2 e
+  float* mass;
+  int64_t meta_page, meta_head;
+  float2* part;                  // [CTAs][2][tiles * 128] (maximum, sum) of a run's unfinished heads
+  float* lse;                    // [batch][kv][tiles * 128] base 2, of heads that one run held whole
+  int* err;
+};
+
+// A maximum over no scores (or over -inf alone) as 0: 2^(-inf - 0) is then 0 without a branch.
+__device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w, int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(tc::smem_u32(dst)),
+      "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// A CTA's run of the line of key tiles, one head at a time.
+struct Run {
+  int b, h, t, n, tiles;  // the current head, its first tile of the run, the sequence's length and tiles
+  int64_t left;           // tiles of the run from there on
+  __device__ void load(const ObserveArgs& a) {
+    n = paged::clamp_length(a.lengths[b], a.width, a.page);
+    tiles = (n + kTile - 1) / kTile;
+  }
+  __device__ int count() const { return (int)min(left, (int64_t)(tiles - t)); }
+  __device__ void next(const ObserveArgs& a) {
+    left -= count();
+    t = 0;
+    if (left == 0 || ++h < a.kv) return;
+    h = 0;
+    do {
+      ++b;
+      load(a);
+    } while (tiles == 0);
   }
 };
 
-template <bool F16, int D>
-__device__ __forceinline__ float dot(const uint16_t* row, const float2 (&q)[D / 64], int lane) {
-  float s = 0.f;
-  if (row != nullptr)
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const float2 x = pair_f32<F16>(*reinterpret_cast<const uint32_t*>(row + 64 * i + 2 * lane));
-      s += q[i].x * x.x + q[i].y * x.y;
-    }
-  return warp_sum(s);
-}
+template <int D, bool F16, int PASS>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_observe_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                         const ObserveArgs a) {
+  using S = Shape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* keys = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* queries = keys + S::kKeys * S::kBytes;
+  __shared__ uint64_t k_full[S::kKeys], k_empty[S::kKeys], q_full[S::kQueries], q_empty[S::kQueries], s_full[4], s_empty[4],
+      drain;
+  __shared__ float2 s_stat[PASS == 1 ? 2 : 1][PASS == 1 ? kMaxTiles * kTile : 1];
+  __shared__ float s_lse[PASS == 2 ? kMaxTiles * kTile : 1];
+  __shared__ int s_place[PASS == 2 ? kMaxTiles * kTile : 1];
+  __shared__ int64_t s_sum[kThreads / 32], s_off;
+  __shared__ int s_seq;
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  paged::launch_next();
 
-template <bool F16, int D>
-__device__ __forceinline__ void load_q(const uint16_t* q, float scale, float2 (&out)[D / 64], int lane) {
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const float2 x = pair_f32<F16>(*reinterpret_cast<const uint32_t*>(q + 64 * i + 2 * lane));
-    out[i] = make_float2(x.x * scale, x.y * scale);
+  if (tid == 0) {
+    for (int s = 0; s < S::kKeys; ++s) tc::mbar_init(&k_full[s], 1), tc::mbar_init(&k_empty[s], 1);
+    for (int s = 0; s < S::kQueries; ++s) tc::mbar_init(&q_full[s], 1), tc::mbar_init(&q_empty[s], 1);
+    for (int s = 0; s < 4; ++s) tc::mbar_init(&s_full[s], 1), tc::mbar_init(&s_empty[s], kGroup);
+    tc::mbar_init(&drain, 1);
+    abort_flag = 0;
+    s_seq = -1;
+    tc::fence_barrier_init();
+    tc::prefetch_tmap(&mq);
+    tc::prefetch_tmap(&mk);
   }
-}
+  if (warp == 1) {
+    tc::tmem_alloc(&tmem_base, kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  paged::wait_previous();
 
-template <bool F16, int D>
-__global__ void __launch_bounds__(32 * kWarps)
-    paged_observe_kernel(const pbk_paged_cache c, const pbk_paged_batch b, const pbk_paged_observe_desc a, int log_page) {
-  __shared__ float sm_m[kWarps], sm_l[kWarps];
-  const int h = blockIdx.x, s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = paged::clamp_length(b.lengths[s], b.width, c.page);
-  const int groups = a.h / c.kv;
-  const Rows r{static_cast<const uint16_t*>(c.k_pages), nullptr, b.block_table + s * b.table_stride, c.stride_page,
-               c.stride_entry, h * c.stride_head, log_page, c.pages, c.page - 1};
-  for (int w0 = 0; w0 < a.queries * groups; ++w0) {
-    const int w = w0 / groups, j = h * groups + w0 % groups, end = n - a.queries + w + 1;
-    if (end <= 0) continue;
-    float2 q[D / 64];
-    load_q<F16, D>(static_cast<const uint16_t*>(a.q) + s * a.q_stride_b + w * a.q_stride_t + j * a.q_stride_h, a.scale, q, lane);
-    float m = -INFINITY, l = 0.f;
-    for (int e = warp; e < end; e += kWarps) {
-      const float x = dot<F16, D>(r.at(r.k, e), q, lane);
-      const float up = fmaxf(m, x);
-      l = l * expf(m - finite(up)) + expf(x - finite(up));
-      m = up;
-    }
-    if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
-    for (int i = 0; i < kWarps; ++i) top = fmaxf(top, sm_m[i]);
-    for (int i = 0; i < kWarps; ++i) total += sm_l[i] * expf(sm_m[i] - finite(top));
-    if (total != 0.f)
-      for (int e = warp; e < end; e += kWarps) {
-        const float x = dot<F16, D>(r.at(r.k, e), q, lane);
-        const int page = paged::page_of(r.table, e, log_page, c.pages);
-        if (lane == 0 && page >= 0)
-          c.mass[page * c.meta_page + h * c.meta_head + (e & r.pmask)] += expf(x - (finite(top) + logf(total)));
+  // ---- this CTA's run: a scan of the sequences' tiles
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+  auto tiles_of = [&](int b) {
+    return (paged::clamp_length(a.lengths[b], a.width, a.page) + kTile - 1) / kTile;
+  };
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+  int64_t before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  if (lane == 31) s_sum[warp] = before;
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  before -= mine;
+  int64_t total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  total *= a.kv;
+  const int64_t length = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1), from = length * blockIdx.x;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t t = tiles_of(b);
+    if (from >= before * a.kv && from < (before + t) * a.kv) s_seq = b, s_off = from - before * a.kv;
+    before += t;
+  }
+  __syncthreads();
+  Run run;
+  run.left = max((int64_t)0, min(length, total - from));
+  run.b = max(s_seq, 0);
+  run.load(a);
+  run.h = run.left > 0 ? (int)(s_off / run.tiles) : 0;
+  run.t = run.left > 0 ? (int)(s_off % run.tiles) : 0;
+
+  auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = tc::globaltimer_ns();
+    while (!tc::mbar_try_wait(bar, parity))
+      if (abort_flag || tc::globaltimer_ns() - t0 > 2000000000ull) {
+        if (a.err) atomicCAS(a.err, 0, 420 + site);
+        abort_flag = 1;
+        return false;
       }
-    __syncthreads();
+    return true;
+  };
+  const bool one = a.tiles == 1;  // the row tile stays for all of a head's key tiles
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    const int rows = min(a.page, kTile), boxes = kTile / rows;  // entries per box, boxes per 64 elements
+    uint32_t kt = 0, qt = 0;
+    bool ok = true;
+    auto load_queries = [&](int b, int h, int rt) -> bool {
+      const uint32_t s = qt % S::kQueries, r = qt / S::kQueries;
+      ++qt;
+      if (r > 0 && !__all_sync(0xffffffffu, wait(&q_empty[s], (r - 1) & 1, 1))) return false;
+      if (lane == 0) {
+        tc::mbar_expect_tx(&q_full[s], a.nw * a.groups * D * 2);
+        for (int i = 0; i < D / 64; ++i)
+          tma_load_5d(queries + s * S::kBytes + i * S::kBlock, &mq, &q_full[s], 0, i, h * a.groups, a.w0 + rt * a.nw, b);
+      }
+      return true;
+    };
+    for (; ok && run.left > 0; run.next(a)) {
+      if (one) ok = load_queries(run.b, run.h, 0);
+      const int32_t* table = a.table + run.b * a.table_stride;
+      const int end = run.t + run.count();
+      for (int t = run.t; ok && t < end; ++t) {
+        const uint32_t s = kt % S::kKeys, r = kt / S::kKeys;
+        ++kt;
+        if (r > 0 && !__all_sync(0xffffffffu, wait(&k_empty[s], (r - 1) & 1, 2))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) tc::mbar_expect_tx(&k_full[s], S::kBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          const int e = t * kTile + lane * rows;
+          const int id = e < run.n ? table[e >> a.log_page] : -1;  // past the length: zeros
+          for (int i = 0; i < D / 64; ++i)
+            tma_load_5d(keys + s * S::kBytes + i * S::kBlock + lane * rows * 128, &mk, &k_full[s], 0, e & (a.page - 1), i,
+                        run.h, id);
+        }
+        for (int rt = 0; ok && !one && rt < a.tiles; ++rt) ok = load_queries(run.b, run.h, rt);
+      }
+    }
+    // the loads issued here land before the CTA's shared memory is given up
+    if (lane == 0) {
+      for (uint32_t i = kt > S::kKeys ? kt - S::kKeys : 0; i < kt; ++i)
+        tc::mbar_wait(&k_full[i % S::kKeys], (i / S::kKeys) & 1, 200000000ull);
+      for (uint32_t i = qt > S::kQueries ? qt - S::kQueries : 0; i < qt; ++i)
+        tc::mbar_wait(&q_full[i % S::kQueries], (i / S::kQueries) & 1, 200000000ull);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t fmt = F16 ? 0u : 1u;
+      const int n = PASS == 1 ? kTile : (a.nw * a.groups + 15) / 16 * 16;
+      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+      uint32_t kt = 0, qt = 0, used[2] = {0, 0};
+      bool ok = true;
+      for (; ok && run.left > 0; run.next(a)) {
+        const int end = run.t + run.count();
+        for (int t = run.t; ok && t < end; ++t, ++kt) {
+          const uint32_t ks = kt % S::kKeys, group = kt & 1;
+          if (!wait(&k_full[ks], (kt / S::kKeys) & 1, 3)) {
+            ok = false;
+            break;
+          }
+          for (int rt = 0; rt < a.tiles; ++rt) {
+            const uint32_t qs = qt % S::kQueries;
+            if ((!one || t == run.t) && !wait(&q_full[qs], (qt / S::kQueries) & 1, 4)) {
+              ok = false;
+              break;
+            }
+            const uint32_t u = used[group]++, buf = group * 2 + (u & 1);
+            if (u >= 2 && !wait(&s_empty[buf], ((u >> 1) - 1) & 1, 5)) {
+              ok = false;
+              break;
+            }
+            tc::fence_after_sync();
+            const uint32_t kb = tc::smem_u32(keys + ks * S::kBytes), qb = tc::smem_u32(queries + qs * S::kBytes);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * S::kBlock + (kk & 3) * 32;
+              const uint64_t kd = tc::sdesc_sw128(kb + off, 16, 1024), qd = tc::sdesc_sw128(qb + off, 16, 1024);
+              tc::mma_f16(tmem + buf * kTile, PASS == 1 ? qd : kd, PASS == 1 ? kd : qd, idesc, kk != 0);
+            }
+            tc::mma_commit(&s_full[buf]);
+            if (!one || t + 1 == end) {
+              tc::mma_commit(&q_empty[qs]);
+              ++qt;
+            }
+          }
+          if (ok) tc::mma_commit(&k_empty[ks]);
+        }
+      }
+      tc::mma_commit(&drain);  // every MMA issued here completes before the CTA exits
+      tc::mbar_wait(&drain, 0, 200000000ull);
+    }
+  } else {
+    // ------------------------------------------------------------ the two epilogue groups
+    const int group = (warp - 2) >> 2, quad = warp & 3, me = quad * 32 + lane;  // a row (pass 1) or an entry (pass 2)
+    const int et = tid - 64;                                                 // 0 .. 255 over both groups
+    const int rows = a.tiles * kTile;
+    uint32_t kt = 0, used = 0;
+    bool ok = true;
+    auto take = [&](uint32_t& taddr) -> bool {  // the group's next accumulator
+      const uint32_t buf = group * 2 + (used & 1);
+      if (!__all_sync(0xffffffffu, wait(&s_full[buf], (used >> 1) & 1, 6))) return false;
+      tc::fence_after_sync();
+      taddr = tmem + ((uint32_t)(quad * 32) << 16) + buf * kTile;
+      return true;
+    };
+    auto give = [&]() {
+      tc::fence_before_sync();
+      tc::mbar_arrive(&s_empty[group * 2 + (used & 1)]);
+      ++used;
+    };
+    // the place in the sequence of row r of the launch: its token's entry; -1 when it has none
+    auto place = [&](int r) {
+      const int w = r / kTile * a.nw + r % kTile / a.groups;
+      return r % kTile < a.nw * a.groups && a.w0 + w < a.queries ? max(run.n - a.queries + a.w0 + w, -1) : -1;
+    };
+    for (; run.left > 0; run.next(a)) {
+      const int count = run.count(), end = run.t + count;
+      const int64_t head = (int64_t)run.b * a.kv + run.h;
+      if (PASS == 1) {
+        for (int r = et; r < 2 * rows; r += 256) s_stat[r / rows][r % rows] = make_float2(-INFINITY, 0.f);
+        group_sync();
+      } else {
+        group_sync();  // the last head's logarithms have been read
+        // the runs that hold this head, from its first tile in the line
+        const int64_t first = from + min(length, total - from) - run.left - run.t;
+        const int run0 = (int)(first / length), run1 = (int)((first + run.tiles - 1) / length);
+        for (int r = et; r < rows; r += 256) {
+          float lse = -INFINITY;
+          if (place(r) >= 0) {
+            if (run0 == run1) {
+              lse = a.lse[head * rows + r];
+            } else {
+              float top = -INFINITY, sum = 0.f;
+              for (int i = run0; i <= run1; ++i) {
+                const float2 x = a.part[((int64_t)i * 2 + (i == run0 ? 1 : 0)) * rows + r];
+                const float up = fmaxf(top, x.x);
+                sum = sum * ex2((top - finite(up)) * a.c) + x.y * ex2((x.x - finite(up)) * a.c);
+                top = up;
+              }
+              lse = finite(top) * a.c + log2f(sum);
+            }
+          }
+          s_lse[r] = lse == -INFINITY ? INFINITY : lse;  // a row without weight adds 0
+          s_place[r] = place(r);
+        }
+        group_sync();
+      }
+      for (int t = run.t; ok && t < end; ++t, ++kt) {
+        if ((int)(kt & 1) != group) continue;
+        const int e0 = t * kTile;
+        const bool whole = e0 + kTile <= run.n - a.queries + 1;  // every row with a place sees all of the tile
+        if (PASS == 1) {
+          for (int rt = 0; rt < a.tiles; ++rt) {
+            uint32_t taddr;
+            if (!(ok = take(taddr))) break;
+            const int end_col = whole ? kTile : min(kTile, place(rt * kTile + me) + 1 - e0);  // columns the row sees
+            float2 ml = s_stat[group][rt * kTile + me];
+            uint32_t x[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tc::tmem_ld_32x32(taddr + 32 * i, x[i]);
+            tc::tmem_ld_wait();
+            give();
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (!whole && 32 * i + j >= end_col) x[i][j] = 0xff800000u;  // -inf
+                top = fmaxf(top, __uint_as_float(x[i][j]));
+              }
+            const float up = fmaxf(ml.x, top), mc = finite(up) * a.c;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[i] += ex2(__uint_as_float(x[i][j]) * a.c - mc);
+            ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            ml.x = up;
+            s_stat[group][rt * kTile + me] = ml;
+          }
+        } else {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int rt = 0; rt < a.tiles; ++rt) {
+            uint32_t taddr;
+            if (!(ok = take(taddr))) break;
+            const int valid = min(a.nw, a.queries - a.w0 - rt * a.nw) * a.groups;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (32 * i >= valid) break;
+              uint32_t x[32];
+              tc::tmem_ld_32x32(taddr + 32 * i, x);
+              tc::tmem_ld_wait();
+              const float* lse = s_lse + rt * kTile + 32 * i;
+              const int* at = s_place + rt * kTile + 32 * i;
+              if (whole && 32 * i + 32 <= valid) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[j & 3] += ex2(__uint_as_float(x[j]) * a.c - lse[j]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  const float y = ex2(__uint_as_float(x[j]) * a.c - lse[j]);
+                  sum[j & 3] += e0 + me <= at[j] ? y : 0.f;
+                }
+              }
+            }
+            give();
+          }
+          if (!ok) break;
+          const int e = e0 + me;
+          if (e < run.n) {
+            const int page = paged::page_of(a.table + run.b * a.table_stride, e, a.log_page, a.pages);
+            if (page >= 0)
+              a.mass[page * a.meta_page + run.h * a.meta_head + (e & (a.page - 1))] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          }
+        }
+      }
+      if (PASS == 1) {
+        group_sync();
+        float2* part = a.part + ((int64_t)blockIdx.x * 2 + (run.t == 0 ? 1 : 0)) * rows;
+        for (int r = et; r < rows; r += 256) {
+          const float2 x = s_stat[0][r], y = s_stat[1][r];
+          const float up = fmaxf(x.x, y.x);
+          const float sum = x.y * ex2((x.x - finite(up)) * a.c) + y.y * ex2((y.x - finite(up)) * a.c);
+          if (count == run.tiles) a.lse[head * rows + r] = finite(up) * a.c + log2f(sum);
+          else part[r] = make_float2(up, sum);
+        }
+        group_sync();
+      }
+    }
   }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+constexpr size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+struct Plan {
+  int groups, nw, row_tiles, ctas;  // row tiles of the whole call
+  size_t lse, bytes;
+};
+
+Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d) {
+  Plan p;
+  p.groups = d.h / c.kv;
+  p.nw = kTile / p.groups < d.queries ? kTile / p.groups : d.queries;
+  p.row_tiles = (d.queries + p.nw - 1) / p.nw;
+  const int64_t tiles = ((int64_t)b.width * c.page + kTile - 1) / kTile * b.batch * c.kv;
+  const int sms = paged_sm_count();
+  p.ctas = (int)(tiles < 1 ? 1 : tiles < sms ? tiles : sms);
+  const int rows = (p.row_tiles < kMaxTiles ? p.row_tiles : kMaxTiles) * kTile;
+  p.lse = align256((size_t)p.ctas * 2 * rows * sizeof(float2));
+  p.bytes = p.lse + align256((size_t)b.batch * c.kv * rows * sizeof(float));
+  return p;
+}
+
+template <int D, bool F16, int PASS>
+cudaError_t launch_pass(const ObserveArgs& a, int ctas, const CUtensorMap& mq, const CUtensorMap& mk, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  auto* kernel = paged_observe_kernel<D, F16, PASS>;
+  const cudaError_t e = paged_allow_smem((const void*)kernel, Shape<D>::kSmem, done);
+  if (e != cudaSuccess) return e;
+  return launch_after(kernel, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, st, 1, mq, mk, a);
+}
+
+template <int D, bool F16>
+cudaError_t launch(const ObserveArgs& a, int ctas, const CUtensorMap& mq, const CUtensorMap& mk, cudaStream_t st) {
+  const cudaError_t e = launch_pass<D, F16, 1>(a, ctas, mq, mk, st);
+  return e != cudaSuccess ? e : launch_pass<D, F16, 2>(a, ctas, mq, mk, st);
 }
 
 }  // namespace
 
-size_t paged_observe_workspace(const pbk_paged_cache&, const pbk_paged_batch&, const pbk_paged_observe_desc&) { return 0; }
+size_t paged_observe_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d) {
+  return make_plan(c, b, d).bytes;
+}
 
 cudaError_t launch_paged_observe(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d,
-                                 void*, cudaStream_t st) {
-  const dim3 grid(c.kv, b.batch);
-  const int lp = paged_log2(c.page);
-  if (c.dtype == PBK_F16) {
-    if (c.d == 64) paged_observe_kernel<true, 64><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
-    else if (c.d == 128) paged_observe_kernel<true, 128><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
-    else paged_observe_kernel<true, 256><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
-  } else {
-    if (c.d == 64) paged_observe_kernel<false, 64><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
-    else if (c.d == 128) paged_observe_kernel<false, 128><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
-    else paged_observe_kernel<false, 256><<<grid, 32 * kWarps, 0, st>>>(c, b, d, lp);
+                                 void* ws, cudaStream_t st) {
+  const Plan p = make_plan(c, b, d);
+  ObserveArgs a = {};
+  a.table = b.block_table, a.table_stride = b.table_stride, a.lengths = b.lengths;
+  a.batch = b.batch, a.width = b.width, a.page = c.page, a.log_page = paged_log2(c.page), a.pages = c.pages;
+  a.kv = c.kv, a.groups = p.groups, a.queries = d.queries, a.nw = p.nw;
+  a.c = d.scale * 1.4426950408889634f;
+  a.mass = c.mass, a.meta_page = c.meta_page, a.meta_head = c.meta_head;
+  a.part = static_cast<float2*>(ws);
+  a.lse = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + p.lse);
+  a.err = device_error_word();
+  CUtensorMap mq, mk;
+  const uint64_t blocks = (uint64_t)(c.d / 64);
+  // queries [64 elements][64-element blocks][heads][queries][sequences]; box: the heads of a key head x nw queries
+  const uint64_t q_dims[5] = {64, blocks, (uint64_t)d.h, (uint64_t)d.queries, (uint64_t)b.batch};
+  const uint64_t q_strides[4] = {128, (uint64_t)d.q_stride_h * 2, (uint64_t)d.q_stride_t * 2, (uint64_t)d.q_stride_b * 2};
+  const uint32_t q_box[5] = {64, 1, (uint32_t)p.groups, (uint32_t)p.nw, 1};
+  // keys [64 elements][entries of a page][64-element blocks][heads][pages]; box: the entries of a page (at most 128)
+  const uint64_t k_dims[5] = {64, (uint64_t)c.page, blocks, (uint64_t)c.kv, (uint64_t)c.pages};
+  const uint64_t k_strides[4] = {(uint64_t)c.stride_entry * 2, 128, (uint64_t)c.stride_head * 2,
+                                 (uint64_t)c.stride_page * 2};
+  const uint32_t k_box[5] = {64, (uint32_t)(c.page < kTile ? c.page : kTile), 1, 1, 1};
+  if (!make_tmap_bf16_sw128(&mq, d.q, 5, q_dims, q_strides, q_box) ||
+      !make_tmap_bf16_sw128(&mk, c.k_pages, 5, k_dims, k_strides, k_box))
+    return cudaErrorInvalidValue;
+  const bool f16 = c.dtype == PBK_F16;
+  for (int t = 0; t < p.row_tiles; t += kMaxTiles) {
+    a.w0 = t * p.nw;
+    a.tiles = p.row_tiles - t < kMaxTiles ? p.row_tiles - t : kMaxTiles;
+    cudaError_t e;
+    if (c.d == 64) e = f16 ? launch<64, true>(a, p.ctas, mq, mk, st) : launch<64, false>(a, p.ctas, mq, mk, st);
+    else if (c.d == 128) e = f16 ? launch<128, true>(a, p.ctas, mq, mk, st) : launch<128, false>(a, p.ctas, mq, mk, st);
+    else e = f16 ? launch<256, true>(a, p.ctas, mq, mk, st) : launch<256, false>(a, p.ctas, mq, mk, st);
+    if (e != cudaSuccess) return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 }  // namespace pbk
