@@ -738,7 +738,7 @@ PBK_API int pbk_paged_observe(const pbk_paged_cache* cache, const pbk_paged_batc
  * below it that become free: src (those entries) and dst (those places), both ascending, the
  * n-th to the n-th, and count [batch, kv]. src and dst are [batch, kv, moves] with moves at
  * least min(budget, capacity - budget) (capacity = width * page; less is PBK_ERR_SHAPE); places
- * past count hold -1. After the moves the sequence has `budget` entries, in no particular
+ * past count hold -1. A row of the table holds at most 2^23 entries. After the moves the sequence has `budget` entries, in no particular
  * order. sinks + recent <= budget. */
 PBK_API size_t pbk_paged_select_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget);
 PBK_API int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget,

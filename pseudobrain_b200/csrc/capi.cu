@@ -905,6 +905,7 @@ int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
   if (st != PBK_OK) return st;
   if (budget < 1 || recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget || moves < 0) return PBK_ERR_INVALID;
   if (batch->batch == 0) return PBK_OK;
+  if ((int64_t)batch->width * cache->page > (1 << 23)) return PBK_ERR_SHAPE;  // the choice's masks in shared memory
   const int64_t past = (int64_t)batch->width * cache->page - budget;
   if (moves < (past < budget ? past : budget)) return PBK_ERR_SHAPE;
   if (!batch->seen || !count || (moves > 0 && (!src || !dst))) return PBK_ERR_INVALID;

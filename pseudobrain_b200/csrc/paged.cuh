@@ -65,15 +65,18 @@ inline int paged_sm_count() {
   return n;
 }
 
-// The dynamic shared memory limit of a kernel, set once per device (bit dev of `done`).
-inline cudaError_t paged_allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+// An attribute of a kernel, set once per device (bit dev of `done`).
+inline cudaError_t paged_allow(const void* kernel, cudaFuncAttribute what, int value, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  e = cudaFuncSetAttribute(kernel, what, value);
   if (e == cudaSuccess && dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   return e;
+}
+inline cudaError_t paged_allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  return paged_allow(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, done);
 }
 
 inline int paged_log2(int x) {

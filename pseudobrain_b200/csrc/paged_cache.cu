@@ -86,98 +86,276 @@ __device__ __forceinline__ uint32_t select_key(float mass, int pos, int sinks, i
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kBins = 2048;          // a digit of 11 bits
+constexpr int kMostKeys = 32768;     // keys that a CTA keeps in shared memory
+constexpr int kMaxCluster = 16;
 
-// One CTA per (sequence, key head): a radix select of the budget-th key, eight bits at a time,
-// then one pass in entry order that ranks the free places and the kept entries past the budget.
-__global__ void __launch_bounds__(kSelThreads)
+// Exclusive prefix of x over the CTA's THREADS threads; the sum in *total. Two uses of `scratch`
+// need a __syncthreads between them.
+template <int THREADS>
+__device__ __forceinline__ uint32_t cta_prefix(uint32_t x, uint32_t* scratch, uint32_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t y = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
+  }
+  if (lane == 31) scratch[warp] = y;
+  __syncthreads();
+  const uint32_t z = lane < THREADS / 32 ? scratch[lane] : 0u;
+  *total = __reduce_add_sync(0xffffffffu, z);
+  return __reduce_add_sync(0xffffffffu, lane < warp ? z : 0u) + y - x;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t x;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(x));
+  return x;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word (four words) of CTA `rank`'s shared memory, at the place that `p` has in this CTA's.
+__device__ __forceinline__ uint32_t remote_at(const uint32_t* p, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(at)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ uint32_t remote(const uint32_t* p, uint32_t rank) {
+  uint32_t x;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(remote_at(p, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ uint4 remote4(const uint32_t* p, uint32_t rank) {
+  uint4 x;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "r"(remote_at(p, rank))
+               : "memory");
+  return x;
+}
+
+// The choice for one (sequence, key head) by a cluster of CTAs, each with an equal share of the
+// entries in order, whose keys it computes once and keeps in shared memory (KEEP; longer shares
+// compute them again in each pass).
+//   1. Three digits of 11, 11 and 10 bits: a histogram of the keys that match the digits so far,
+//      summed over the cluster (each CTA sums its part of the bins, all read the sums), from whose
+//      top the budget-th key's digit follows.
+//   2. Two bit masks per 32 entries: above the budget-th key, and equal to it; of the equal ones
+//      the lowest entries of the whole cluster stay until the budget is full.
+//   3. Prefix sums over the masks, in the CTA and over the cluster, give every free place below
+//      the budget and every kept entry past it its rank in the answer.
+// Bound by latency: three histograms and five cluster barriers for a share of some thousand
+// entries (8 bytes each), against 1 us for the bytes.
+template <int THREADS, bool KEEP>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
     paged_select_kernel(const pbk_paged_cache c, const pbk_paged_batch b, int budget, int recent, int sinks,
-                        int32_t* src, int32_t* dst, int32_t* count, int moves, int log_page) {
+                        int32_t* src, int32_t* dst, int32_t* count, int moves, int log_page, int ctas, int share) {
+  extern __shared__ __align__(16) uint32_t smem[];
+  uint32_t* hist = smem;                            // [3][kBins] of this CTA's entries
+  uint32_t* sums = hist + 3 * kBins;                // [3][kBins] the cluster's, of this CTA's bins; not for one CTA
+  uint32_t* masks = sums + (ctas > 1 ? 3 * kBins : 0);  // [share / 32][2]
+  uint32_t* keys = masks + share / 16;              // [share], 16-byte aligned: share is a multiple of 64
+  __shared__ uint32_t scratch[THREADS / 32], found[2], counts[2];
   paged::launch_next();
   paged::wait_previous();
-  const int h = blockIdx.x, s = blockIdx.y;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t orow = (int64_t)s * c.kv + h;
-  int32_t* osrc = src + orow * moves;
-  int32_t* odst = dst + orow * moves;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x / ctas, h = pair % c.kv, s = pair / c.kv;
   const int n = paged::clamp_length(b.lengths[s], b.width, c.page);
+  int32_t* osrc = src + (int64_t)pair * moves;
+  int32_t* odst = dst + (int64_t)pair * moves;
+  if (n <= budget) {  // the whole cluster
+    if (rank == 0 && tid == 0) count[pair] = 0;
+    for (int i = rank * THREADS + tid; i < moves; i += ctas * THREADS) osrc[i] = odst[i] = -1;
+    return;
+  }
   const int32_t* table = b.block_table + s * b.table_stride;
   const int64_t first_recent = (int64_t)b.seen[s] - recent;
-  int done = 0;
-  if (n > budget) {
-    auto key_of = [&](int j) -> uint32_t {
-      const int page = paged::page_of(table, j, log_page, c.pages);
-      float m = 0.f;
-      int p = -1;
-      if (page >= 0) {
-        const int64_t at = page * c.meta_page + h * c.meta_head + (j & (c.page - 1));
-        m = c.mass[at];
-        p = c.pos[at];
-      }
-      return select_key(m, p, sinks, first_recent);
-    };
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need;
-    if (tid == 0) s_prefix = 0, s_need = budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      const uint32_t prefix = s_prefix;
-      const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-      for (int j = tid; j < n; j += kSelThreads) {
-        const uint32_t key = key_of(j);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int need = s_need, bin = 255;
-        while (bin > 0 && (int)hist[bin] < need) need -= hist[bin--];
-        s_need = need;
-        s_prefix = prefix | ((uint32_t)bin << shift);
-      }
-      __syncthreads();
+  // an equal share of 32-entry words per CTA (share is the most, by the table's capacity)
+  const int words = (n + 31) / 32, per = (words + ctas - 1) / ctas;
+  const int w0 = min((int)rank * per, words), w1 = min(w0 + per, words), e0 = 32 * w0, mine = min(32 * w1, n) - e0;
+
+  // the four keys from entry e0 + i on (i a multiple of 4); past the share's end 0
+  auto load_keys = [&](int i) -> uint4 {
+    const int e = e0 + i;
+    const int id = paged::page_of(table, e, log_page, c.pages), page = max(id, 0);  // no branch between loads
+    const int64_t at = page * c.meta_page + h * c.meta_head + (e & (c.page - 1));
+    float4 m = *reinterpret_cast<const float4*>(c.mass + at);
+    int4 p = *reinterpret_cast<const int4*>(c.pos + at);
+    if (id < 0) m = make_float4(0.f, 0.f, 0.f, 0.f), p = make_int4(-1, -1, -1, -1);
+    uint4 k;
+    k.x = select_key(m.x, p.x, sinks, first_recent);
+    k.y = i + 1 < mine ? select_key(m.y, p.y, sinks, first_recent) : 0u;
+    k.z = i + 2 < mine ? select_key(m.z, p.z, sinks, first_recent) : 0u;
+    k.w = i + 3 < mine ? select_key(m.w, p.w, sinks, first_recent) : 0u;
+    return k;
+  };
+  for (int i = tid; i < (ctas > 1 ? 6 : 3) * kBins; i += THREADS) hist[i] = 0;  // and the sums
+  if (KEEP) {
+    // all of a thread's loads of a turn are in flight together
+    constexpr int kEach = 4;
+    for (int i0 = 4 * tid; i0 < mine; i0 += 4 * kEach * THREADS) {
+      uint4 k[kEach];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) k[j] = load_keys(min(i0 + 4 * j * THREADS, (mine - 1) & ~3));
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (i0 + 4 * j * THREADS < mine) *reinterpret_cast<uint4*>(keys + i0 + 4 * j * THREADS) = k[j];
     }
-    const uint32_t bar = s_prefix;  // the budget-th key; s_need of the entries equal to it stay
-    const int need = s_need;
-    __shared__ int wsum[32];
-    int eq_run = 0, hole_run = 0, move_run = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-      const int j = j0 + tid;
-      const uint32_t key = j < n ? key_of(j) : 0u;
-      const bool eq = j < n && key == bar;
-      const uint32_t eq_bal = __ballot_sync(0xffffffffu, eq);
-      if (lane == 0) wsum[warp] = __popc(eq_bal);
-      __syncthreads();
-      int before = 0, total = 0;
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) before += wsum[w];
-        total += wsum[w];
-      }
-      __syncthreads();
-      const int eq_rank = eq_run + before + __popc(eq_bal & ((1u << lane) - 1u));
-      const bool kept = j < n && (key > bar || (eq && eq_rank < need));
-      eq_run += total;
-      const bool hole = j < budget && !kept, mover = j >= budget && kept;
-      const uint32_t h_bal = __ballot_sync(0xffffffffu, hole), m_bal = __ballot_sync(0xffffffffu, mover);
-      if (lane == 0) wsum[warp] = __popc(h_bal) | (__popc(m_bal) << 16);
-      __syncthreads();
-      before = total = 0;
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) before += wsum[w];
-        total += wsum[w];
-      }
-      __syncthreads();
-      const uint32_t below = (1u << lane) - 1u;
-      if (hole) odst[hole_run + (before & 0xFFFF) + __popc(h_bal & below)] = j;
-      if (mover) osrc[move_run + (before >> 16) + __popc(m_bal & below)] = j;
-      hole_run += total & 0xFFFF;
-      move_run += total >> 16;
-    }
-    done = hole_run;
   }
-  if (tid == 0) count[orow] = done;
-  for (int i = done + tid; i < moves; i += kSelThreads) osrc[i] = odst[i] = -1;
+  __syncthreads();
+  uint32_t prefix = 0, need = (uint32_t)budget;  // the digits so far; how many of the keys that match them stay
+#pragma unroll 1
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+    uint32_t* hst = hist + digit * kBins;
+    const uint32_t above = digit == 0 ? 0u : prefix >> (shift + bits);
+    for (int i0 = 0; i0 < mine; i0 += 4 * THREADS) {
+      const int i = i0 + 4 * tid;
+      uint4 k = make_uint4(0u, 0u, 0u, 0u);
+      if (i < mine) {
+        if (KEEP) k = *reinterpret_cast<const uint4*>(keys + i);
+        else k = load_keys(i);
+      }
+      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
+      uint32_t bin[4];
+      bool take[4], all = true, any = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bin[j] = (kk[j] >> shift) & ((1u << bits) - 1u);
+        take[j] = i + j < mine && (digit == 0 || (kk[j] >> (shift + bits)) == above);
+        all = all && take[j] && bin[j] == bin[0];
+        any = any || take[j];
+      }
+      if (!__any_sync(0xffffffffu, any)) continue;
+      // many entries may share a key (protected ones, those without weight yet): a warp whose 128
+      // agree counts them at once
+      const uint32_t first = __shfl_sync(0xffffffffu, bin[0], 0);
+      if (__all_sync(0xffffffffu, all && bin[0] == first)) {
+        if (lane == 0) atomicAdd(&hst[bin[0]], 128u);
+      } else if (all) {
+        atomicAdd(&hst[bin[0]], 4u);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (take[j]) atomicAdd(&hst[bin[j]], 1u);
+      }
+    }
+    // the cluster's sums: this CTA's kBins / ctas bins, each by as many threads as there are for it
+    const int part = kBins / ctas, log_ctas = 31 - __clz(ctas);
+    uint32_t* sum_of = sums + digit * kBins;
+    if (ctas == 1) {
+      __syncthreads();
+    } else {
+      cluster_sync();
+      for (int i = tid; i < 4 * part; i += THREADS) {  // a quarter of the CTAs each
+        const int bin = i % part, q = i / part;
+        uint32_t x = 0;
+#pragma unroll 4
+        for (int r = q; r < ctas; r += 4) x += remote(hst + rank * part + bin, r);
+        if (x != 0) atomicAdd(&sum_of[bin], x);
+      }
+      cluster_sync();
+    }
+    // bins from the top, kBins / THREADS per thread; the thread whose bins reach `need` tells
+    constexpr int kPer = kBins / THREADS;
+    const int low = kBins - kPer * (tid + 1), owner = low >> (11 - log_ctas);
+    uint32_t bins[kPer], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const int at = low + kPer - 4 - j;
+      const uint4 x = ctas == 1 ? *reinterpret_cast<const uint4*>(hst + at) : remote4(sum_of + (at & (part - 1)), owner);
+      bins[j] = x.w, bins[j + 1] = x.z, bins[j + 2] = x.y, bins[j + 3] = x.x;
+      sum += (x.x + x.y) + (x.z + x.w);
+    }
+    uint32_t before = cta_prefix<THREADS>(sum, scratch, &total);
+    if (before < need && before + sum >= need) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (before < need && before + bins[j] >= need) {
+          found[0] = prefix | ((uint32_t)(low + kPer - 1 - j) << shift);
+          found[1] = need - before;
+        }
+        before += bins[j];
+      }
+    }
+    __syncthreads();
+    prefix = found[0], need = found[1];
+    __syncthreads();
+  }
+  // prefix is the budget-th key; `need` of the entries equal to it stay, the lowest first
+  const uint32_t equal_before =
+      __reduce_add_sync(0xffffffffu, lane < (int)rank ? remote(hist + 2 * kBins + (prefix & 1023u), lane) : 0u);
+  for (int w = tid >> 5; w < w1 - w0; w += (THREADS / 32)) {
+    const int i = 32 * w + lane;
+    uint32_t k = 0;
+    if (i < mine) {
+      if (KEEP) {
+        k = keys[i];
+      } else {
+        const uint4 q = load_keys(i & ~3);
+        k = (i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w;
+      }
+    }
+    const uint32_t gt = __ballot_sync(0xffffffffu, i < mine && k > prefix);
+    const uint32_t eq = __ballot_sync(0xffffffffu, i < mine && k == prefix);
+    if (lane == 0) masks[2 * w] = gt, masks[2 * w + 1] = eq;
+  }
+  __syncthreads();
+  // a thread per word, in turns: kept entries, then the ranks of free places and movers; the first
+  // round counts for the cluster, the second writes
+  const int turns = (w1 - w0 + THREADS - 1) / THREADS;
+  uint32_t equal_run = equal_before, holes = 0, movers = 0;
+  for (int turn = 0; turn < turns; ++turn) {
+    const int w = turn * THREADS + tid;
+    uint32_t gt = 0, eq = 0, total;
+    if (w < w1 - w0) gt = masks[2 * w], eq = masks[2 * w + 1];
+    const uint32_t at = equal_run + cta_prefix<THREADS>((uint32_t)__popc(eq), scratch, &total);
+    equal_run += total;
+    __syncthreads();
+    if (w < w1 - w0) {
+      const int stay = at >= need ? 0 : min((int)(need - at), __popc(eq));
+      uint32_t kept = gt, rest = eq;
+      for (int i = 0; i < stay; ++i) kept |= rest & (0u - rest), rest &= rest - 1u;
+      // entries below the budget that go, and at or past it that stay
+      const int first = e0 + 32 * w;
+      const uint32_t exist = n - first >= 32 ? 0xFFFFFFFFu : (1u << (n - first)) - 1u;
+      const uint32_t low = budget <= first ? 0u : budget - first >= 32 ? 0xFFFFFFFFu : (1u << (budget - first)) - 1u;
+      masks[2 * w] = ~kept & exist & low;
+      masks[2 * w + 1] = kept & ~low;
+      holes += (uint32_t)__popc(masks[2 * w]), movers += (uint32_t)__popc(masks[2 * w + 1]);
+    }
+  }
+  uint32_t all_holes, all_movers;
+  cta_prefix<THREADS>(holes, scratch, &all_holes);
+  __syncthreads();
+  cta_prefix<THREADS>(movers, scratch, &all_movers);
+  if (tid == 0) counts[0] = all_holes, counts[1] = all_movers;
+  cluster_sync();
+  const uint32_t theirs = lane < ctas ? remote(counts, lane) : 0u, moved = lane < ctas ? remote(counts + 1, lane) : 0u;
+  const uint32_t done = __reduce_add_sync(0xffffffffu, theirs);
+  uint32_t hole_run = __reduce_add_sync(0xffffffffu, lane < (int)rank ? theirs : 0u);
+  uint32_t move_run = __reduce_add_sync(0xffffffffu, lane < (int)rank ? moved : 0u);
+  cluster_sync();  // no CTA leaves while another reads its counts
+  for (int turn = 0; turn < turns; ++turn) {
+    const int w = turn * THREADS + tid;
+    uint32_t hole = 0, mover = 0, total;
+    if (w < w1 - w0) hole = masks[2 * w], mover = masks[2 * w + 1];
+    uint32_t at = hole_run + cta_prefix<THREADS>((uint32_t)__popc(hole), scratch, &total);
+    hole_run += total;
+    __syncthreads();
+    for (; hole != 0; hole &= hole - 1u) odst[at++] = e0 + 32 * w + __ffs(hole) - 1;
+    at = move_run + cta_prefix<THREADS>((uint32_t)__popc(mover), scratch, &total);
+    move_run += total;
+    __syncthreads();
+    for (; mover != 0; mover &= mover - 1u) osrc[at++] = e0 + 32 * w + __ffs(mover) - 1;
+  }
+  if (rank == 0 && tid == 0) count[pair] = (int)done;
+  for (int i = (int)done + rank * THREADS + tid; i < moves; i += ctas * THREADS) osrc[i] = odst[i] = -1;
 }
 
 }  // namespace
@@ -196,8 +374,28 @@ size_t paged_select_workspace(const pbk_paged_cache&, const pbk_paged_batch&, in
 
 cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
                                 int32_t* src, int32_t* dst, int32_t* count, int moves, void*, cudaStream_t st) {
-  return launch_after(paged_select_kernel, dim3(c.kv, b.batch), dim3(kSelThreads), 0, st, 1, c, b, budget, recent, sinks, src,
-                      dst, count, moves, paged_log2(c.page));
+  // CTAs per (sequence, key head): more while a share holds over 2048 entries and the grid has
+  // room on the SMs, and as many as it takes to keep the shares in shared memory
+  const int64_t pairs = (int64_t)b.batch * c.kv, cap = (int64_t)b.width * c.page;
+  int ctas = 1;
+  while (ctas < kMaxCluster && ((cap > 2048 * ctas && pairs * 2 * ctas <= 2 * paged_sm_count()) || cap > (int64_t)kMostKeys * ctas))
+    ctas *= 2;
+  const int64_t words = (cap + 31) / 32, share = ((words + ctas - 1) / ctas + 1) / 2 * 64;
+  const bool keep = share <= kMostKeys;
+  const int64_t smem = (ctas > 1 ? 6 : 3) * kBins * 4 + share / 4 + (keep ? share * 4 : 0);
+  static std::atomic<uint64_t> done[3][2];
+  // long shares have more threads, many short ones more CTAs per SM
+  const int which = !keep ? 2 : share > 4608 ? 1 : 0;
+  auto* kernel = which == 2 ? paged_select_kernel<512, false> : which == 1 ? paged_select_kernel<512, true>
+                                                                          : paged_select_kernel<256, true>;
+  cudaError_t e = paged_allow((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024, done[which][0]);
+  if (e == cudaSuccess && ctas > 8)
+    e = paged_allow((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, done[which][1]);
+  if (e != cudaSuccess) return e;
+  pbk_paged_batch used = b;
+  if (c.pages == 0) used.width = 0;  // no pages, no entries
+  return launch_after(kernel, dim3((unsigned)(pairs * ctas)), dim3(which == 0 ? 256 : 512), (int)smem, st, ctas, c, used,
+                      budget, recent, sinks, src, dst, count, moves, paged_log2(c.page), ctas, (int)share);
 }
 
 cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
