@@ -12,10 +12,11 @@
 //
 // Keys are cut into tiles of 128 entries of one (sequence, key head); all tiles stand in one line
 // and each CTA (one per SM) takes an equal run of it. Row tiles hold as many whole queries as fit
-// 128 rows; up to kMaxTiles of them share each key tile, more take further launches. Warps: 0
-// TMA producer (keys page by page, queries as one box of heads x queries), 1 MMA issuer, 2-5 and
-// 6-9 two groups that take alternate key tiles from four accumulators in TMEM. Every wait is
-// bounded; on timeout the kernel records an error code and winds down.
+// 128 rows; up to kMaxTiles of them share each key tile, more take further launches. Warps: 0 and
+// 10 TMA producers (a key tile is up to 64 boxes, page by page, and one warp issues a box in
+// about 45 ns; queries come as one box of heads x queries), 1 MMA issuer, 2-5 and 6-9 two groups
+// that take alternate key tiles from four accumulators in TMEM. Every wait is bounded; on timeout
+// the kernel records an error code and winds down.
 //
 // What bounds it: per key tile and pass 128 x 128 exponentials (16 a clock and SM: 0.55 us), the
 // keys' bytes (32 KB at an SM's share of HBM: 0.75 us) and 0.37 us of MMA.
@@ -31,16 +32,20 @@ namespace {
 
 constexpr int kTile = 128;       // entries of a key tile, rows of a row tile
 constexpr int kMaxTiles = 8;     // row tiles of a launch
-constexpr int kThreads = 320;
+constexpr int kProducers = 2;    // producer warps: warp 0 and the one after the epilogue's
+constexpr int kThreads = 320 + 32 * (kProducers - 1);
 constexpr int kGroup = 128;      // threads of an epilogue group
 constexpr uint32_t kTmemCols = 512;
 
-template <int D>
+// Stages of the key and query rings. One row tile (ONE) stays for all of a head's key tiles, and
+// the keys get what is left: a saturated HBM takes some 4 us to answer, which 192 KB in flight
+// per SM just cover. More row tiles pass by once per key tile, out of L2.
+template <int D, bool ONE>
 struct Shape {
   static constexpr int kBytes = kTile * D * 2;  // a tile of keys or queries
   static constexpr int kBlock = kTile * 128;    // its 64-element columns: 128 rows of 128 bytes
-  static constexpr int kKeys = D == 64 ? 6 : D == 128 ? 3 : 2;
-  static constexpr int kQueries = D == 256 ? 1 : 2;
+  static constexpr int kKeys = ONE ? (D == 64 ? 12 : D == 128 ? 6 : 2) : (D == 64 ? 5 : D == 128 ? 3 : 1);
+  static constexpr int kQueries = ONE ? 1 : D == 64 ? 5 : D == 128 ? 3 : 2;
   static constexpr int kSmem = (kKeys + kQueries) * kBytes + 1024;
 };
 
@@ -66,6 +71,33 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations in one instruction (fma.rn.f32x2 and add.rn.f32x2 round each half like the
+// scalar ones).
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^(x c + d) of two scores.
+__device__ __forceinline__ uint64_t exp_pair(uint32_t x0, uint32_t x1, uint64_t c, uint64_t d) {
+  const float2 y = unpack2(fma2(pack2(__uint_as_float(x0), __uint_as_float(x1)), c, d));
+  return pack2(ex2(y.x), ex2(y.y));
+}
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
                                             int w, int v) {
   asm volatile(
@@ -74,42 +106,66 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, u
       "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
       : "memory");
 }
+// Waits for this thread's TMEM loads and ties the registers to the wait.
+__device__ __forceinline__ void landed(uint32_t (&x)[32]) {
+  tc::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(x[i]));
+}
 __device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// A CTA's run of the line of key tiles, one head at a time.
+// A CTA's run of the line of key tiles, one head at a time. Pass 2 walks it backwards: what pass
+// 1 read last is what L2 still holds.
+template <int PASS>
 struct Run {
-  int b, h, t, n, tiles;  // the current head, its first tile of the run, the sequence's length and tiles
-  int64_t left;           // tiles of the run from there on
+  int b, h, t, n, tiles, count;  // the head, its tiles t .. t + count - 1 of the run; the sequence's length and tiles
+  int64_t left;                  // tiles of the run from this head on, its own among them
   __device__ void load(const ObserveArgs& a) {
     n = paged::clamp_length(a.lengths[b], a.width, a.page);
     tiles = (n + kTile - 1) / kTile;
   }
-  __device__ int count() const { return (int)min(left, (int64_t)(tiles - t)); }
-  __device__ void next(const ObserveArgs& a) {
-    left -= count();
-    t = 0;
-    if (left == 0 || ++h < a.kv) return;
-    h = 0;
-    do {
-      ++b;
-      load(a);
-    } while (tiles == 0);
+  // `at`: the first tile of the run in its head (pass 1), the last one (pass 2)
+  __device__ void start(const ObserveArgs& a, int b_, int64_t at, int64_t length) {
+    b = b_, left = length, h = t = count = 0;
+    load(a);
+    if (left == 0) return;
+    h = (int)(at / tiles);
+    place((int)(at % tiles));
   }
+  __device__ void place(int at) {
+    if (PASS == 1) t = at, count = (int)min(left, (int64_t)(tiles - at));
+    else count = (int)min(left, (int64_t)(at + 1)), t = at + 1 - count;
+  }
+  __device__ void next(const ObserveArgs& a) {
+    left -= count;
+    if (left == 0) return;
+    if (PASS == 1 ? ++h == a.kv : --h < 0) {
+      h = PASS == 1 ? 0 : a.kv - 1;
+      do {
+        b += PASS == 1 ? 1 : -1;
+        load(a);
+      } while (tiles == 0);
+    }
+    place(PASS == 1 ? 0 : tiles - 1);
+  }
+  __device__ int tile(int i) const { return PASS == 1 ? t + i : t + count - 1 - i; }  // the i-th to be taken
 };
 
-template <int D, bool F16, int PASS>
+template <int D, bool F16, bool ONE, int PASS>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_observe_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                          const ObserveArgs a) {
-  using S = Shape<D>;
+  using S = Shape<D, ONE>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* keys = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* queries = keys + S::kKeys * S::kBytes;
   __shared__ uint64_t k_full[S::kKeys], k_empty[S::kKeys], q_full[S::kQueries], q_empty[S::kQueries], s_full[4], s_empty[4],
       drain;
-  __shared__ float2 s_stat[PASS == 1 ? 2 : 1][PASS == 1 ? kMaxTiles * kTile : 1];
-  __shared__ float s_lse[PASS == 2 ? kMaxTiles * kTile : 1];
-  __shared__ int s_place[PASS == 2 ? kMaxTiles * kTile : 1];
+  constexpr int kRows = ONE ? kTile : kMaxTiles * kTile;
+  // pass 1: the groups' (maximum, sum) per row; of one row tile the second group's, at the end
+  __shared__ float2 s_stat[PASS == 1 && !ONE ? 2 : 1][PASS == 1 ? kRows : 1];
+  __shared__ __align__(16) float s_lse[PASS == 2 ? kRows : 4];  // pass 2: negated
+  __shared__ int s_place[PASS == 2 ? kRows : 1];
   __shared__ int64_t s_sum[kThreads / 32], s_off;
   __shared__ int s_seq;
   __shared__ uint32_t tmem_base;
@@ -161,18 +217,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   total *= a.kv;
   const int64_t length = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1), from = length * blockIdx.x;
+  const int64_t mine_tiles = max((int64_t)0, min(length, total - from)), seek = PASS == 1 ? from : from + mine_tiles - 1;
   for (int b = b0; b < b1; ++b) {
     const int64_t t = tiles_of(b);
-    if (from >= before * a.kv && from < (before + t) * a.kv) s_seq = b, s_off = from - before * a.kv;
+    if (mine_tiles > 0 && seek >= before * a.kv && seek < (before + t) * a.kv) s_seq = b, s_off = seek - before * a.kv;
     before += t;
   }
   __syncthreads();
-  Run run;
-  run.left = max((int64_t)0, min(length, total - from));
-  run.b = max(s_seq, 0);
-  run.load(a);
-  run.h = run.left > 0 ? (int)(s_off / run.tiles) : 0;
-  run.t = run.left > 0 ? (int)(s_off % run.tiles) : 0;
+  Run<PASS> run;
+  run.start(a, max(s_seq, 0), mine_tiles > 0 ? s_off : 0, mine_tiles);
 
   auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
     if (tc::mbar_try_wait(bar, parity)) return true;
@@ -185,11 +238,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     return true;
   };
-  const bool one = a.tiles == 1;  // the row tile stays for all of a head's key tiles
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    const int rows = min(a.page, kTile), boxes = kTile / rows;  // entries per box, boxes per 64 elements
+  if (warp == 0 || warp >= 10) {
+    // ------------------------------------------------------------ TMA producers
+    const int producer = warp == 0 ? 0 : warp - 9;
+    const int rows = min(a.page, kTile);  // entries per box
+    // this lane's box of every key tile: a page's entries, 64 elements of the head
+    const int box = lane * kProducers + producer, at = box / (D / 64) * rows, block = box % (D / 64);
+    const bool mine = at < kTile;
     uint32_t kt = 0, qt = 0;
     bool ok = true;
     auto load_queries = [&](int b, int h, int rt) -> bool {
@@ -203,31 +259,37 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return true;
     };
-    for (; ok && run.left > 0; run.next(a)) {
-      if (one) ok = load_queries(run.b, run.h, 0);
-      const int32_t* table = a.table + run.b * a.table_stride;
-      const int end = run.t + run.count();
-      for (int t = run.t; ok && t < end; ++t) {
+    // the page of this lane's box in tile t (-1 past the length: zeros); read a tile ahead, since
+    // a load from the table takes as long as an SM's share of a tile
+    auto page_id = [&](const Run<PASS>& r, int t) {
+      const int e = t * kTile + at;
+      return mine && e < r.n ? a.table[r.b * a.table_stride + (e >> a.log_page)] : -1;
+    };
+    int id = run.left > 0 ? page_id(run, run.tile(0)) : -1;
+    while (ok && run.left > 0) {
+      if (ONE && producer == 0) ok = load_queries(run.b, run.h, 0);
+      const Run<PASS> head = run;
+      run.next(a);
+      for (int i = 0; ok && i < head.count; ++i) {
+        const int now = id, e = head.tile(i) * kTile + at;
+        if (i + 1 < head.count) id = page_id(head, head.tile(i + 1));
+        else if (run.left > 0) id = page_id(run, run.tile(0));
         const uint32_t s = kt % S::kKeys, r = kt / S::kKeys;
         ++kt;
         if (r > 0 && !__all_sync(0xffffffffu, wait(&k_empty[s], (r - 1) & 1, 2))) {
           ok = false;
           break;
         }
-        if (lane == 0) tc::mbar_expect_tx(&k_full[s], S::kBytes);
-        __syncwarp();
-        if (lane < boxes) {
-          const int e = t * kTile + lane * rows;
-          const int id = e < run.n ? table[e >> a.log_page] : -1;  // past the length: zeros
-          for (int i = 0; i < D / 64; ++i)
-            tma_load_5d(keys + s * S::kBytes + i * S::kBlock + lane * rows * 128, &mk, &k_full[s], 0, e & (a.page - 1), i,
-                        run.h, id);
-        }
-        for (int rt = 0; ok && !one && rt < a.tiles; ++rt) ok = load_queries(run.b, run.h, rt);
+        // (another producer's boxes may land first: the phase ends only after this arrival)
+        if (producer == 0 && lane == 0) tc::mbar_expect_tx(&k_full[s], S::kBytes);
+        if (mine)
+          tma_load_5d(keys + s * S::kBytes + block * S::kBlock + at * 128, &mk, &k_full[s], 0, e & (a.page - 1), block, head.h,
+                      now);
+        for (int rt = 0; ok && !ONE && producer == 0 && rt < a.tiles; ++rt) ok = load_queries(head.b, head.h, rt);
       }
     }
     // the loads issued here land before the CTA's shared memory is given up
-    if (lane == 0) {
+    if (producer == 0 && lane == 0) {
       for (uint32_t i = kt > S::kKeys ? kt - S::kKeys : 0; i < kt; ++i)
         tc::mbar_wait(&k_full[i % S::kKeys], (i / S::kKeys) & 1, 200000000ull);
       for (uint32_t i = qt > S::kQueries ? qt - S::kQueries : 0; i < qt; ++i)
@@ -239,42 +301,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t fmt = F16 ? 0u : 1u;
       const int n = PASS == 1 ? kTile : (a.nw * a.groups + 15) / 16 * 16;
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
-      uint32_t kt = 0, qt = 0, used[2] = {0, 0};
+      // the descriptors of the rings' first stages; a stage and a K step add to the address field
+      // (bits 0-13, 16-byte units)
+      const uint64_t k_desc = tc::sdesc_sw128(tc::smem_u32(keys), 16, 1024);
+      const uint64_t q_desc = tc::sdesc_sw128(tc::smem_u32(queries), 16, 1024);
+      uint32_t kt = 0, ks = 0, k_phase = 0, qs = 0, q_phase = 0;
       bool ok = true;
       for (; ok && run.left > 0; run.next(a)) {
-        const int end = run.t + run.count();
-        for (int t = run.t; ok && t < end; ++t, ++kt) {
-          const uint32_t ks = kt % S::kKeys, group = kt & 1;
-          if (!wait(&k_full[ks], (kt / S::kKeys) & 1, 3)) {
-            ok = false;
-            break;
-          }
-          for (int rt = 0; rt < a.tiles; ++rt) {
-            const uint32_t qs = qt % S::kQueries;
-            if ((!one || t == run.t) && !wait(&q_full[qs], (qt / S::kQueries) & 1, 4)) {
-              ok = false;
-              break;
-            }
-            const uint32_t u = used[group]++, buf = group * 2 + (u & 1);
-            if (u >= 2 && !wait(&s_empty[buf], ((u >> 1) - 1) & 1, 5)) {
-              ok = false;
-              break;
-            }
+        if (ONE) ok = wait(&q_full[0], q_phase, 4);
+        for (int left = run.count; ok && left > 0; --left, ++kt) {
+          ok = wait(&k_full[ks], k_phase, 3);
+          for (int rt = 0; ok && rt < a.tiles; ++rt) {
+            if (!ONE && !(ok = wait(&q_full[qs], q_phase, 4))) break;
+            const uint32_t u = (kt >> 1) * a.tiles + rt, buf = (kt & 1) * 2 + (u & 1);  // the group's u-th product
+            if (u >= 2 && !(ok = wait(&s_empty[buf], ((u >> 1) - 1) & 1, 5))) break;
             tc::fence_after_sync();
-            const uint32_t kb = tc::smem_u32(keys + ks * S::kBytes), qb = tc::smem_u32(queries + qs * S::kBytes);
+            const uint64_t kd0 = k_desc + ks * (S::kBytes >> 4), qd0 = q_desc + qs * (S::kBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * S::kBlock + (kk & 3) * 32;
-              const uint64_t kd = tc::sdesc_sw128(kb + off, 16, 1024), qd = tc::sdesc_sw128(qb + off, 16, 1024);
-              tc::mma_f16(tmem + buf * kTile, PASS == 1 ? qd : kd, PASS == 1 ? kd : qd, idesc, kk != 0);
+              const uint32_t off = ((kk >> 2) * S::kBlock + (kk & 3) * 32) >> 4;
+              tc::mma_f16(tmem + buf * kTile, PASS == 1 ? qd0 + off : kd0 + off, PASS == 1 ? kd0 + off : qd0 + off, idesc,
+                          kk != 0);
             }
             tc::mma_commit(&s_full[buf]);
-            if (!one || t + 1 == end) {
+            if (!ONE) {
               tc::mma_commit(&q_empty[qs]);
-              ++qt;
+              if (++qs == S::kQueries) qs = 0, q_phase ^= 1;
             }
           }
           if (ok) tc::mma_commit(&k_empty[ks]);
+          if (++ks == S::kKeys) ks = 0, k_phase ^= 1;
+        }
+        if (ONE && ok) {
+          tc::mma_commit(&q_empty[0]);
+          q_phase ^= 1;
         }
       }
       tc::mma_commit(&drain);  // every MMA issued here completes before the CTA exits
@@ -305,15 +365,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       return r % kTile < a.nw * a.groups && a.w0 + w < a.queries ? max(run.n - a.queries + a.w0 + w, -1) : -1;
     };
     for (; run.left > 0; run.next(a)) {
-      const int count = run.count(), end = run.t + count;
       const int64_t head = (int64_t)run.b * a.kv + run.h;
+      float2 ml = make_float2(-INFINITY, 0.f);  // pass 1, ONE: this thread's row
       if (PASS == 1) {
-        for (int r = et; r < 2 * rows; r += 256) s_stat[r / rows][r % rows] = make_float2(-INFINITY, 0.f);
+        if (!ONE)
+          for (int r = et; r < 2 * rows; r += 256) s_stat[r / rows][r % rows] = ml;
         group_sync();
       } else {
         group_sync();  // the last head's logarithms have been read
         // the runs that hold this head, from its first tile in the line
-        const int64_t first = from + min(length, total - from) - run.left - run.t;
+        const int64_t first = from + run.left - run.count - run.t;
         const int run0 = (int)(first / length), run1 = (int)((first + run.tiles - 1) / length);
         for (int r = et; r < rows; r += 256) {
           float lse = -INFINITY;
@@ -331,88 +392,116 @@ __global__ void __launch_bounds__(kThreads, 1)
               lse = finite(top) * a.c + log2f(sum);
             }
           }
-          s_lse[r] = lse == -INFINITY ? INFINITY : lse;  // a row without weight adds 0
+          s_lse[r] = lse == -INFINITY ? -INFINITY : -lse;  // a row without weight adds 0
           s_place[r] = place(r);
         }
         group_sync();
       }
-      for (int t = run.t; ok && t < end; ++t, ++kt) {
+      int id = -1;  // pass 2: the page of this thread's entry, read a turn of the group ahead
+      auto page_id = [&](int i) {
+        if (PASS == 1 || i >= run.count) return -1;
+        const int e = run.tile(i) * kTile + me;
+        return e < run.n ? paged::page_of(a.table + run.b * a.table_stride, e, a.log_page, a.pages) : -1;
+      };
+      id = page_id((int)(kt & 1) == group ? 0 : 1);
+      for (int i = 0; ok && i < run.count; ++i, ++kt) {
         if ((int)(kt & 1) != group) continue;
-        const int e0 = t * kTile;
+        const int t = run.tile(i), e0 = t * kTile;
         const bool whole = e0 + kTile <= run.n - a.queries + 1;  // every row with a place sees all of the tile
+        float* to = nullptr;
+        float have = 0.f;
+        if (PASS == 2) {
+          if (id >= 0) {
+            to = a.mass + id * a.meta_page + run.h * a.meta_head + ((e0 + me) & (a.page - 1));
+            have = *to;
+          }
+          id = page_id(i + 2);
+        }
         if (PASS == 1) {
           for (int rt = 0; rt < a.tiles; ++rt) {
             uint32_t taddr;
             if (!(ok = take(taddr))) break;
             const int end_col = whole ? kTile : min(kTile, place(rt * kTile + me) + 1 - e0);  // columns the row sees
-            float2 ml = s_stat[group][rt * kTile + me];
+            if (!ONE) ml = s_stat[group][rt * kTile + me];
             uint32_t x[4][32];
 #pragma unroll
             for (int i = 0; i < 4; ++i) tc::tmem_ld_32x32(taddr + 32 * i, x[i]);
-            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) landed(x[i]);
             give();
-            float top = -INFINITY;
+            if (!whole)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (!whole && 32 * i + j >= end_col) x[i][j] = 0xff800000u;  // -inf
-                top = fmaxf(top, __uint_as_float(x[i][j]));
-              }
-            const float up = fmaxf(ml.x, top), mc = finite(up) * a.c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 32; ++j)
+                  if (32 * i + j >= end_col) x[i][j] = 0xff800000u;  // -inf
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 32; j += 2)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sum[i] += ex2(__uint_as_float(x[i][j]) * a.c - mc);
-            ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+              for (int i = 0; i < 4; ++i)
+                top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[i][j])), __uint_as_float(x[i][j + 1]));
+            const float up = fmaxf(ml.x, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), mc = finite(up) * a.c;
+            const uint64_t c2 = pack2(a.c, a.c), d2 = pack2(-mc, -mc);
+            uint64_t sum[4] = {0, 0, 0, 0};  // pairs of zeros
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[i] = add2(sum[i], exp_pair(x[i][j], x[i][j + 1], c2, d2));
+            const float2 part = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+            ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + (part.x + part.y);
             ml.x = up;
-            s_stat[group][rt * kTile + me] = ml;
+            if (!ONE) s_stat[group][rt * kTile + me] = ml;
           }
         } else {
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint64_t sum[4] = {0, 0, 0, 0};  // pairs of zeros
+          const uint64_t c2 = pack2(a.c, a.c);
           for (int rt = 0; rt < a.tiles; ++rt) {
             uint32_t taddr;
             if (!(ok = take(taddr))) break;
             const int valid = min(a.nw, a.queries - a.w0 - rt * a.nw) * a.groups;
+            uint32_t x[2][32];  // a chunk of 32 rows is on its way while the one before it is summed
+            tc::tmem_ld_32x32(taddr, x[0]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (32 * i >= valid) break;
-              uint32_t x[32];
-              tc::tmem_ld_32x32(taddr + 32 * i, x);
-              tc::tmem_ld_wait();
-              const float* lse = s_lse + rt * kTile + 32 * i;
+              landed(x[i & 1]);
+              if (i < 3 && 32 * i + 32 < valid) tc::tmem_ld_32x32(taddr + 32 * i + 32, x[(i + 1) & 1]);
+              const ulonglong2* d4 = reinterpret_cast<const ulonglong2*>(s_lse + rt * kTile + 32 * i);
               const int* at = s_place + rt * kTile + 32 * i;
+              const uint32_t(&y)[32] = x[i & 1];
               if (whole && 32 * i + 32 <= valid) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[j & 3] += ex2(__uint_as_float(x[j]) * a.c - lse[j]);
+                for (int j = 0; j < 8; ++j) {
+                  const ulonglong2 d = d4[j];
+                  sum[2 * (j & 1)] = add2(sum[2 * (j & 1)], exp_pair(y[4 * j], y[4 * j + 1], c2, d.x));
+                  sum[2 * (j & 1) + 1] = add2(sum[2 * (j & 1) + 1], exp_pair(y[4 * j + 2], y[4 * j + 3], c2, d.y));
+                }
               } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                  const float y = ex2(__uint_as_float(x[j]) * a.c - lse[j]);
-                  sum[j & 3] += e0 + me <= at[j] ? y : 0.f;
+                  const float w = ex2(__uint_as_float(y[j]) * a.c + s_lse[rt * kTile + 32 * i + j]);
+                  sum[j & 3] = add2(sum[j & 3], pack2(e0 + me <= at[j] ? w : 0.f, 0.f));
                 }
               }
             }
             give();
           }
           if (!ok) break;
-          const int e = e0 + me;
-          if (e < run.n) {
-            const int page = paged::page_of(a.table + run.b * a.table_stride, e, a.log_page, a.pages);
-            if (page >= 0)
-              a.mass[page * a.meta_page + run.h * a.meta_head + (e & (a.page - 1))] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          }
+          const float2 part = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+          if (to != nullptr) *to = have + (part.x + part.y);
         }
       }
       if (PASS == 1) {
+        if (ONE && group == 1) s_stat[0][me] = ml;
         group_sync();
         float2* part = a.part + ((int64_t)blockIdx.x * 2 + (run.t == 0 ? 1 : 0)) * rows;
-        for (int r = et; r < rows; r += 256) {
-          const float2 x = s_stat[0][r], y = s_stat[1][r];
+        for (int r = ONE ? me : et; r < rows; r += 256) {
+          if (ONE && group == 1) break;
+          const float2 x = ONE ? ml : s_stat[0][r], y = ONE ? s_stat[0][r] : s_stat[ONE ? 0 : 1][r];
           const float up = fmaxf(x.x, y.x);
           const float sum = x.y * ex2((x.x - finite(up)) * a.c) + y.y * ex2((y.x - finite(up)) * a.c);
-          if (count == run.tiles) a.lse[head * rows + r] = finite(up) * a.c + log2f(sum);
+          if (run.count == run.tiles) a.lse[head * rows + r] = finite(up) * a.c + log2f(sum);
           else part[r] = make_float2(up, sum);
         }
         group_sync();
@@ -445,19 +534,25 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
   return p;
 }
 
-template <int D, bool F16, int PASS>
+template <int D, bool F16, bool ONE, int PASS>
 cudaError_t launch_pass(const ObserveArgs& a, int ctas, const CUtensorMap& mq, const CUtensorMap& mk, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  auto* kernel = paged_observe_kernel<D, F16, PASS>;
-  const cudaError_t e = paged_allow_smem((const void*)kernel, Shape<D>::kSmem, done);
+  auto* kernel = paged_observe_kernel<D, F16, ONE, PASS>;
+  const cudaError_t e = paged_allow_smem((const void*)kernel, Shape<D, ONE>::kSmem, done);
   if (e != cudaSuccess) return e;
-  return launch_after(kernel, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, st, 1, mq, mk, a);
+  return launch_after(kernel, dim3((unsigned)ctas), dim3(kThreads), Shape<D, ONE>::kSmem, st, 1, mq, mk, a);
+}
+
+template <int D, bool F16, bool ONE>
+cudaError_t launch_passes(const ObserveArgs& a, int ctas, const CUtensorMap& mq, const CUtensorMap& mk, cudaStream_t st) {
+  const cudaError_t e = launch_pass<D, F16, ONE, 1>(a, ctas, mq, mk, st);
+  return e != cudaSuccess ? e : launch_pass<D, F16, ONE, 2>(a, ctas, mq, mk, st);
 }
 
 template <int D, bool F16>
 cudaError_t launch(const ObserveArgs& a, int ctas, const CUtensorMap& mq, const CUtensorMap& mk, cudaStream_t st) {
-  const cudaError_t e = launch_pass<D, F16, 1>(a, ctas, mq, mk, st);
-  return e != cudaSuccess ? e : launch_pass<D, F16, 2>(a, ctas, mq, mk, st);
+  return a.tiles == 1 ? launch_passes<D, F16, true>(a, ctas, mq, mk, st)
+                      : launch_passes<D, F16, false>(a, ctas, mq, mk, st);
 }
 
 }  // namespace

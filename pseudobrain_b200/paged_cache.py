@@ -46,6 +46,7 @@ from ._capi import (LIB, PbkPagedAttendDesc, PbkPagedBatch, PbkPagedCache, PbkPa
 
 _DTYPES = {torch.bfloat16: _capi.PBK_BF16, torch.float16: _capi.PBK_F16, torch.float32: _capi.PBK_F32}
 _byref = ctypes.byref
+_INT_MAX = 2 ** 31 - 1
 
 
 @dataclass
@@ -127,15 +128,18 @@ def _call(cache: PagedCache, fn, what: str, *args) -> None:
 
 def _batch(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor | None, seen: torch.Tensor | None = None):
     i = cache._index
-    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != i or table.stride(1) != 1:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != i or (strides := table.stride())[1] != 1:
         raise ValueError("block_table must be int32 [B, M] on the cache's GPU with contiguous rows")
     b, m = table.shape
-    for t, name in ((lengths, "lengths"), (seen, "seen")):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != b or t.get_device() != i
-                              or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32 [{b}] on the cache's GPU")
-    return PbkPagedBatch(b, m, table.data_ptr(), table.stride(0), None if lengths is None else lengths.data_ptr(),
-                         None if seen is None else seen.data_ptr())
+    return PbkPagedBatch(b, m, table.data_ptr(), strides[0],
+                         None if lengths is None else _per_sequence(lengths, "lengths", b, i),
+                         None if seen is None else _per_sequence(seen, "seen", b, i))
+
+
+def _per_sequence(t: torch.Tensor, name: str, b: int, index: int) -> int:
+    if t.dtype != torch.int32 or t.shape != (b,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{b}] on the cache's GPU")
+    return t.data_ptr()
 
 
 def _need(cache: PagedCache, what: str, *names: str) -> None:
@@ -202,15 +206,18 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
     if window is not None and window < 1:
         raise ValueError("paged_attend: the window holds at least the new token (None: no window)")
     n, h, d = q.shape
+    sb, sh, _ = q.stride()
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out, ob, oh = torch.empty_like(q, memory_format=torch.contiguous_format), h * d, d
     elif out.shape != q.shape or out.dtype not in (q.dtype, torch.float32) or out.stride(-1) != 1 \
             or out.device != q.device:
         raise ValueError(f"paged_attend: out must be {tuple(q.shape)}, {q.dtype} or fp32, with a contiguous last dim")
+    else:
+        ob, oh, _ = out.stride()
     lse = torch.empty(n, h, dtype=torch.float32, device=q.device)
-    desc = PbkPagedAttendDesc(h, 0 if window is None else window, sinks, accumulate, d ** -0.5 if scale is None else scale,
-                              _DTYPES[out.dtype], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-                              out.stride(1), lse.data_ptr())
+    desc = PbkPagedAttendDesc(h, 0 if window is None else min(window, _INT_MAX), min(sinks, _INT_MAX), accumulate,
+                              d ** -0.5 if scale is None else scale, _DTYPES[out.dtype], q.data_ptr(), sb, sh, out.data_ptr(), ob,
+                              oh, lse.data_ptr())
     bref, dref = _byref(b), _byref(desc)
     _run(cache, LIB.pbk_paged_attend, "pbk_paged_attend", LIB.pbk_paged_attend_workspace(cache._ref, bref, dref),
          cache._ref, bref, dref)
