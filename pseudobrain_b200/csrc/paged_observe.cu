@@ -93,17 +93,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^(x c + d) of two scores.
-__device__ __forceinline__ uint64_t exp_pair(uint32_t x0, uint32_t x1, uint64_t c, uint64_t d) {
-  const float2 y = unpack2(fma2(pack2(__uint_as_float(x0), __uint_as_float(x1)), c, d));
-  return pack2(ex2(y.x), ex2(y.y));
+// sum[i & 3] += 2^(x c + d) over 16 scores, in three rounds of independent instructions.
+__device__ __forceinline__ void add_exps(uint64_t (&sum)[4], const uint32_t* x, uint64_t c, const uint64_t (&d)[8]) {
+  uint64_t y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c, d[i]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 z = unpack2(y[i]);
+    y[i] = pack2(ex2(z.x), ex2(z.y));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i & 3] = add2(sum[i & 3], y[i]);
+}
+// L2 cache policies: leave first, stay.
+__device__ __forceinline__ uint64_t policy_first() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t policy_last() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
-                                            int w, int v) {
+                                            int w, int v, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
-      "[%2];" ::"r"(tc::smem_u32(dst)),
-      "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(tc::smem_u32(dst)),
+      "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "l"(policy)
       : "memory");
 }
 // Waits for this thread's TMEM loads and ties the registers to the wait.
@@ -114,9 +133,7 @@ __device__ __forceinline__ void landed(uint32_t (&x)[32]) {
 }
 __device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// A CTA's run of the line of key tiles, one head at a time. Pass 2 walks it backwards: what pass
-// 1 read last is what L2 still holds.
-template <int PASS>
+// A CTA's run of the line of key tiles, one head at a time.
 struct Run {
   int b, h, t, n, tiles, count;  // the head, its tiles t .. t + count - 1 of the run; the sequence's length and tiles
   int64_t left;                  // tiles of the run from this head on, its own among them
@@ -124,31 +141,25 @@ struct Run {
     n = paged::clamp_length(a.lengths[b], a.width, a.page);
     tiles = (n + kTile - 1) / kTile;
   }
-  // `at`: the first tile of the run in its head (pass 1), the last one (pass 2)
-  __device__ void start(const ObserveArgs& a, int b_, int64_t at, int64_t length) {
+  __device__ void start(const ObserveArgs& a, int b_, int64_t at, int64_t length) {  // at: its first tile in sequence b_
     b = b_, left = length, h = t = count = 0;
     load(a);
     if (left == 0) return;
-    h = (int)(at / tiles);
-    place((int)(at % tiles));
-  }
-  __device__ void place(int at) {
-    if (PASS == 1) t = at, count = (int)min(left, (int64_t)(tiles - at));
-    else count = (int)min(left, (int64_t)(at + 1)), t = at + 1 - count;
+    h = (int)(at / tiles), t = (int)(at % tiles);
+    count = (int)min(left, (int64_t)(tiles - t));
   }
   __device__ void next(const ObserveArgs& a) {
     left -= count;
     if (left == 0) return;
-    if (PASS == 1 ? ++h == a.kv : --h < 0) {
-      h = PASS == 1 ? 0 : a.kv - 1;
+    if (++h == a.kv) {
+      h = 0;
       do {
-        b += PASS == 1 ? 1 : -1;
+        ++b;
         load(a);
       } while (tiles == 0);
     }
-    place(PASS == 1 ? 0 : tiles - 1);
+    t = 0, count = (int)min(left, (int64_t)tiles);
   }
-  __device__ int tile(int i) const { return PASS == 1 ? t + i : t + count - 1 - i; }  // the i-th to be taken
 };
 
 template <int D, bool F16, bool ONE, int PASS>
@@ -217,14 +228,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   total *= a.kv;
   const int64_t length = max((total + gridDim.x - 1) / gridDim.x, (int64_t)1), from = length * blockIdx.x;
-  const int64_t mine_tiles = max((int64_t)0, min(length, total - from)), seek = PASS == 1 ? from : from + mine_tiles - 1;
+  const int64_t mine_tiles = max((int64_t)0, min(length, total - from));
   for (int b = b0; b < b1; ++b) {
     const int64_t t = tiles_of(b);
-    if (mine_tiles > 0 && seek >= before * a.kv && seek < (before + t) * a.kv) s_seq = b, s_off = seek - before * a.kv;
+    if (mine_tiles > 0 && from >= before * a.kv && from < (before + t) * a.kv) s_seq = b, s_off = from - before * a.kv;
     before += t;
   }
   __syncthreads();
-  Run<PASS> run;
+  Run run;
   run.start(a, max(s_seq, 0), mine_tiles > 0 ? s_off : 0, mine_tiles);
 
   auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
@@ -246,6 +257,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // this lane's box of every key tile: a page's entries, 64 elements of the head
     const int box = lane * kProducers + producer, at = box / (D / 64) * rows, block = box % (D / 64);
     const bool mine = at < kTile;
+    // Keys are read once per pass and leave L2 first; the queries and the masses between them stay
+    // (131072 entries x 8 heads: 121 -> 112 us; asking for part of the keys to stay for pass 2: 117).
+    const uint64_t first = policy_first(), last = policy_last();
     uint32_t kt = 0, qt = 0;
     bool ok = true;
     auto load_queries = [&](int b, int h, int rt) -> bool {
@@ -255,25 +269,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         tc::mbar_expect_tx(&q_full[s], a.nw * a.groups * D * 2);
         for (int i = 0; i < D / 64; ++i)
-          tma_load_5d(queries + s * S::kBytes + i * S::kBlock, &mq, &q_full[s], 0, i, h * a.groups, a.w0 + rt * a.nw, b);
+          tma_load_5d(queries + s * S::kBytes + i * S::kBlock, &mq, &q_full[s], 0, i, h * a.groups, a.w0 + rt * a.nw, b,
+                      last);
       }
       return true;
     };
     // the page of this lane's box in tile t (-1 past the length: zeros); read a tile ahead, since
     // a load from the table takes as long as an SM's share of a tile
-    auto page_id = [&](const Run<PASS>& r, int t) {
+    auto page_id = [&](const Run& r, int t) {
       const int e = t * kTile + at;
       return mine && e < r.n ? a.table[r.b * a.table_stride + (e >> a.log_page)] : -1;
     };
-    int id = run.left > 0 ? page_id(run, run.tile(0)) : -1;
+    int id = run.left > 0 ? page_id(run, run.t) : -1;
     while (ok && run.left > 0) {
       if (ONE && producer == 0) ok = load_queries(run.b, run.h, 0);
-      const Run<PASS> head = run;
+      const Run head = run;
       run.next(a);
       for (int i = 0; ok && i < head.count; ++i) {
-        const int now = id, e = head.tile(i) * kTile + at;
-        if (i + 1 < head.count) id = page_id(head, head.tile(i + 1));
-        else if (run.left > 0) id = page_id(run, run.tile(0));
+        const int now = id, e = (head.t + i) * kTile + at;
+        if (i + 1 < head.count) id = page_id(head, head.t + i + 1);
+        else if (run.left > 0) id = page_id(run, run.t);
         const uint32_t s = kt % S::kKeys, r = kt / S::kKeys;
         ++kt;
         if (r > 0 && !__all_sync(0xffffffffu, wait(&k_empty[s], (r - 1) & 1, 2))) {
@@ -284,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (producer == 0 && lane == 0) tc::mbar_expect_tx(&k_full[s], S::kBytes);
         if (mine)
           tma_load_5d(keys + s * S::kBytes + block * S::kBlock + at * 128, &mk, &k_full[s], 0, e & (a.page - 1), block, head.h,
-                      now);
+                      now, first);
         for (int rt = 0; ok && !ONE && producer == 0 && rt < a.tiles; ++rt) ok = load_queries(head.b, head.h, rt);
       }
     }
@@ -374,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         group_sync();  // the last head's logarithms have been read
         // the runs that hold this head, from its first tile in the line
-        const int64_t first = from + run.left - run.count - run.t;
+        const int64_t first = from + mine_tiles - run.left - run.t;
         const int run0 = (int)(first / length), run1 = (int)((first + run.tiles - 1) / length);
         for (int r = et; r < rows; r += 256) {
           float lse = -INFINITY;
@@ -383,11 +398,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               lse = a.lse[head * rows + r];
             } else {
               float top = -INFINITY, sum = 0.f;
-              for (int i = run0; i <= run1; ++i) {
-                const float2 x = a.part[((int64_t)i * 2 + (i == run0 ? 1 : 0)) * rows + r];
-                const float up = fmaxf(top, x.x);
-                sum = sum * ex2((top - finite(up)) * a.c) + x.y * ex2((x.x - finite(up)) * a.c);
-                top = up;
+              for (int i0 = run0; i0 <= run1; i0 += 8) {  // eight pieces' loads in flight
+                float2 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const int i = min(i0 + k, run1);
+                  x[k] = a.part[((int64_t)i * 2 + (i == run0 ? 1 : 0)) * rows + r];
+                  if (i0 + k > run1) x[k] = make_float2(-INFINITY, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float up = fmaxf(top, x[k].x);
+                  sum = sum * ex2((top - finite(up)) * a.c) + x[k].y * ex2((x[k].x - finite(up)) * a.c);
+                  top = up;
+                }
               }
               lse = finite(top) * a.c + log2f(sum);
             }
@@ -400,13 +424,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       int id = -1;  // pass 2: the page of this thread's entry, read a turn of the group ahead
       auto page_id = [&](int i) {
         if (PASS == 1 || i >= run.count) return -1;
-        const int e = run.tile(i) * kTile + me;
+        const int e = (run.t + i) * kTile + me;
         return e < run.n ? paged::page_of(a.table + run.b * a.table_stride, e, a.log_page, a.pages) : -1;
       };
       id = page_id((int)(kt & 1) == group ? 0 : 1);
       for (int i = 0; ok && i < run.count; ++i, ++kt) {
         if ((int)(kt & 1) != group) continue;
-        const int t = run.tile(i), e0 = t * kTile;
+        const int t = (run.t + i), e0 = t * kTile;
         const bool whole = e0 + kTile <= run.n - a.queries + 1;  // every row with a place sees all of the tile
         float* to = nullptr;
         float have = 0.f;
@@ -442,12 +466,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 4; ++i)
                 top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[i][j])), __uint_as_float(x[i][j + 1]));
             const float up = fmaxf(ml.x, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), mc = finite(up) * a.c;
-            const uint64_t c2 = pack2(a.c, a.c), d2 = pack2(-mc, -mc);
+            const uint64_t c2 = pack2(a.c, a.c), d2 = pack2(-mc, -mc), d[8] = {d2, d2, d2, d2, d2, d2, d2, d2};
             uint64_t sum[4] = {0, 0, 0, 0};  // pairs of zeros
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sum[i] = add2(sum[i], exp_pair(x[i][j], x[i][j + 1], c2, d2));
+            for (int i = 0; i < 8; ++i) add_exps(sum, x[i / 2] + 16 * (i & 1), c2, d);
             const float2 part = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
             ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + (part.x + part.y);
             ml.x = up;
@@ -472,10 +494,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t(&y)[32] = x[i & 1];
               if (whole && 32 * i + 32 <= valid) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const ulonglong2 d = d4[j];
-                  sum[2 * (j & 1)] = add2(sum[2 * (j & 1)], exp_pair(y[4 * j], y[4 * j + 1], c2, d.x));
-                  sum[2 * (j & 1) + 1] = add2(sum[2 * (j & 1) + 1], exp_pair(y[4 * j + 2], y[4 * j + 3], c2, d.y));
+                for (int j = 0; j < 2; ++j) {
+                  uint64_t d[8];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) d[2 * k] = d4[4 * j + k].x, d[2 * k + 1] = d4[4 * j + k].y;
+                  add_exps(sum, y + 16 * j, c2, d);
                 }
               } else {
 #pragma unroll
