@@ -46,35 +46,58 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-__global__ void __launch_bounds__(256)
+// A warp takes 8 moves of one (sequence, key head): 8 lanes look up the moves and their pages, then
+// all lanes copy the 8 key and value rows, D / 16 16-byte chunks each, every load before the first
+// store. Bound by HBM and by how many rows are in flight: a thread per chunk that looks its move
+// up itself took 19.1 us for 57344 moves (71 MB).
+constexpr int kMoves = 8;            // moves per warp
+constexpr int kMoveThreads = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads)
     paged_move_kernel(const pbk_paged_cache c, const pbk_paged_batch b, const int32_t* src, const int32_t* dst,
                       const int32_t* count, int moves, int log_page) {
   paged::launch_next();
   paged::wait_previous();
-  const int h = blockIdx.y, s = blockIdx.z;
-  const int64_t row = (int64_t)s * c.kv + h;
-  const int n = min(count[row], moves);
-  const int chunks = c.d >> 3;
-  const int32_t* table = b.block_table + s * b.table_stride;
-  const int64_t cap = (int64_t)b.width << log_page;
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n * chunks; i += gridDim.x * blockDim.x) {
-    const int ch = i % chunks, j = i / chunks;
-    const int from = src[row * moves + j], to = dst[row * moves + j];
-    if (from < 0 || to < 0 || from >= cap || to >= cap) continue;
-    const int fp = paged::page_of(table, from, log_page, c.pages), tp = paged::page_of(table, to, log_page, c.pages);
-    if (fp < 0 || tp < 0) continue;
-    const int fr = from & (c.page - 1), tr = to & (c.page - 1);
-    const int64_t f = fp * c.stride_page + h * c.stride_head + fr * c.stride_entry + 8 * ch;
-    const int64_t t = tp * c.stride_page + h * c.stride_head + tr * c.stride_entry + 8 * ch;
-    uint16_t* k = reinterpret_cast<uint16_t*>(c.k_pages);
-    uint16_t* v = reinterpret_cast<uint16_t*>(c.v_pages);
-    *reinterpret_cast<uint4*>(k + t) = *reinterpret_cast<const uint4*>(k + f);
-    *reinterpret_cast<uint4*>(v + t) = *reinterpret_cast<const uint4*>(v + f);
-    if (ch == 0) {
-      const int64_t fm = fp * c.meta_page + h * c.meta_head + fr, tm = tp * c.meta_page + h * c.meta_head + tr;
-      if (c.mass != nullptr) c.mass[tm] = c.mass[fm];
-      if (c.pos != nullptr) c.pos[tm] = c.pos[fm];
+  const int h = blockIdx.y, s = blockIdx.z, lane = threadIdx.x & 31;
+  const int64_t row = ((int64_t)s * c.kv + h) * moves;
+  const int n = min(count[(int64_t)s * c.kv + h], moves);
+  const int first = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kMoves;
+  if (first >= n) return;
+  // element offsets of this lane's move (lanes below 8), -1 when there is none
+  int64_t from = -1, to = -1;
+  if (lane < kMoves && first + lane < n) {
+    const int fe = src[row + first + lane], te = dst[row + first + lane];
+    const int64_t cap = (int64_t)b.width << log_page;
+    if (fe >= 0 && te >= 0 && fe < cap && te < cap) {
+      const int32_t* table = b.block_table + s * b.table_stride;
+      const int fp = paged::page_of(table, fe, log_page, c.pages), tp = paged::page_of(table, te, log_page, c.pages);
+      if (fp >= 0 && tp >= 0) {
+        const int fr = fe & (c.page - 1), tr = te & (c.page - 1);
+        from = fp * c.stride_page + h * c.stride_head + fr * c.stride_entry;
+        to = tp * c.stride_page + h * c.stride_head + tr * c.stride_entry;
+        const int64_t fm = fp * c.meta_page + h * c.meta_head + fr, tm = tp * c.meta_page + h * c.meta_head + tr;
+        if (c.mass != nullptr) c.mass[tm] = c.mass[fm];
+        if (c.pos != nullptr) c.pos[tm] = c.pos[fm];
+      }
     }
+  }
+  constexpr int kRow = D / 8, kEach = kMoves * 2 * kRow / 32;  // chunks of a row, chunks per lane
+  uint16_t* k = reinterpret_cast<uint16_t*>(c.k_pages);
+  uint16_t* v = reinterpret_cast<uint16_t*>(c.v_pages);
+  uint4 x[kEach];
+  int64_t at[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int chunk = i * 32 + lane, move = chunk / (2 * kRow), r = chunk % (2 * kRow);
+    const int64_t f = __shfl_sync(0xffffffffu, from, move);
+    at[i] = __shfl_sync(0xffffffffu, to, move);
+    if (f >= 0) x[i] = *reinterpret_cast<const uint4*>((r < kRow ? k : v) + f + r % kRow * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int r = (i * 32 + lane) % (2 * kRow);
+    if (at[i] >= 0) *reinterpret_cast<uint4*>((r < kRow ? k : v) + at[i] + r % kRow * 8) = x[i];
   }
 }
 
@@ -124,6 +147,9 @@ __device__ __forceinline__ uint32_t remote_at(const uint32_t* p, uint32_t rank) 
                : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
   return at;
 }
+__device__ __forceinline__ void remote_add(uint32_t* p, uint32_t rank, uint32_t x) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(remote_at(p, rank)), "r"(x) : "memory");
+}
 __device__ __forceinline__ uint32_t remote(const uint32_t* p, uint32_t rank) {
   uint32_t x;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(remote_at(p, rank)) : "memory");
@@ -142,8 +168,8 @@ __device__ __forceinline__ uint4 remote4(const uint32_t* p, uint32_t rank) {
 // entries in order, whose keys it computes once and keeps in shared memory (KEEP; longer shares
 // compute them again in each pass).
 //   1. Three digits of 11, 11 and 10 bits: a histogram of the keys that match the digits so far,
-//      summed over the cluster (each CTA sums its part of the bins, all read the sums), from whose
-//      top the budget-th key's digit follows.
+//      summed over the cluster (a CTA owns a part of the bins, the others add theirs to it, all read
+//      the sums), from whose top the budget-th key's digit follows.
 //   2. Two bit masks per 32 entries: above the budget-th key, and equal to it; of the equal ones
 //      the lowest entries of the whole cluster stay until the budget is full.
 //   3. Prefix sums over the masks, in the CTA and over the cluster, give every free place below
@@ -207,7 +233,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
         if (i0 + 4 * j * THREADS < mine) *reinterpret_cast<uint4*>(keys + i0 + 4 * j * THREADS) = k[j];
     }
   }
-  __syncthreads();
+  if (ctas > 1) cluster_sync();  // the sums are zero before anyone adds to them
+  else __syncthreads();
   uint32_t prefix = 0, need = (uint32_t)budget;  // the digits so far; how many of the keys that match them stay
 #pragma unroll 1
   for (int digit = 0; digit < 3; ++digit) {
@@ -245,20 +272,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
           if (take[j]) atomicAdd(&hst[bin[j]], 1u);
       }
     }
-    // the cluster's sums: this CTA's kBins / ctas bins, each by as many threads as there are for it
+    __syncthreads();
+    // the cluster's sums: bin i is kept by CTA i / (kBins / ctas)
     const int part = kBins / ctas, log_ctas = 31 - __clz(ctas);
     uint32_t* sum_of = sums + digit * kBins;
-    if (ctas == 1) {
-      __syncthreads();
-    } else {
-      cluster_sync();
-      for (int i = tid; i < 4 * part; i += THREADS) {  // a quarter of the CTAs each
-        const int bin = i % part, q = i / part;
-        uint32_t x = 0;
-#pragma unroll 4
-        for (int r = q; r < ctas; r += 4) x += remote(hst + rank * part + bin, r);
-        if (x != 0) atomicAdd(&sum_of[bin], x);
-      }
+    if (ctas > 1) {
+      for (int i = tid; i < kBins; i += THREADS)
+        if (hst[i] != 0) remote_add(sum_of + (i & (part - 1)), i >> (11 - log_ctas), hst[i]);
       cluster_sync();
     }
     // bins from the top, kBins / THREADS per thread; the thread whose bins reach `need` tells
@@ -400,9 +420,10 @@ cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch&
 
 cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
                               const int32_t* dst, const int32_t* count, int moves, cudaStream_t st) {
-  const int64_t blocks = ((int64_t)moves * (c.d / 8) + 255) / 256;
-  return launch_after(paged_move_kernel, dim3((unsigned)(blocks < 64 ? blocks : 64), c.kv, b.batch), dim3(256), 0, st, 1, c, b, src,
-                      dst, count, moves, paged_log2(c.page));
+  constexpr int kPerBlock = kMoveThreads / 32 * kMoves;
+  const dim3 grid((unsigned)(((int64_t)moves + kPerBlock - 1) / kPerBlock), c.kv, b.batch);
+  auto* kernel = c.d == 64 ? paged_move_kernel<64> : c.d == 128 ? paged_move_kernel<128> : paged_move_kernel<256>;
+  return launch_after(kernel, grid, dim3(kMoveThreads), 0, st, 1, c, b, src, dst, count, moves, paged_log2(c.page));
 }
 
 }  // namespace pbk
