@@ -695,7 +695,9 @@ PBK_API int pbk_paged_append(const pbk_paged_cache* cache, const pbk_paged_batch
  * (lengths after the token was appended; the window counts entries, so it is for a cache
  * whose entries lie in order). A sequence without visible entries gives out 0 and lse -inf.
  * accumulate != 0: mass_i += sum_j p_ji over the key head's query heads. Workspace bytes from
- * pbk_paged_attend_workspace (0 for a desc that the call would reject). */
+ * pbk_paged_attend_workspace (0 for a desc that the call would reject, and where none is
+ * needed); with accumulate they hold a score of 4 bytes per query head and entry that the table
+ * has room for (of the window and sinks alone where there is a window). */
 typedef struct pbk_paged_attend_desc {
   int32_t h, window, sinks, accumulate;
   float scale;
@@ -716,7 +718,7 @@ PBK_API int pbk_paged_attend(const pbk_paged_cache* cache, const pbk_paged_batch
  * query w standing at entry lengths[b] - queries + w (lengths with those tokens appended);
  * entry i is visible to it when i <= that place, and a query whose place is negative adds
  * nothing. mass_i += sum over queries and the key head's query heads of their weights. At
- * most 1024 queries. */
+ * most 1024 queries; q's strides positive. */
 typedef struct pbk_paged_observe_desc {
   int32_t h, queries;
   float scale;

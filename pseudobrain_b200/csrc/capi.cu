@@ -836,6 +836,9 @@ int validate_observe(const pbk_paged_cache* c, const pbk_paged_batch* b, const p
   if (!aligned16(d->q) || !aligned_elems(d->q_stride_b, 8) || !aligned_elems(d->q_stride_t, 8) ||
       !aligned_elems(d->q_stride_h, 8))
     return PBK_ERR_ALIGN;
+  // TMA's strides: positive wherever there is more than one
+  if ((b->batch > 1 && d->q_stride_b <= 0) || (d->queries > 1 && d->q_stride_t <= 0) || (d->h > 1 && d->q_stride_h <= 0))
+    return PBK_ERR_INVALID;
   return PBK_OK;
 }
 

@@ -600,7 +600,8 @@ cudaError_t launch_paged_observe(const pbk_paged_cache& c, const pbk_paged_batch
   const uint64_t blocks = (uint64_t)(c.d / 64);
   // queries [64 elements][64-element blocks][heads][queries][sequences]; box: the heads of a key head x nw queries
   const uint64_t q_dims[5] = {64, blocks, (uint64_t)d.h, (uint64_t)d.queries, (uint64_t)b.batch};
-  const uint64_t q_strides[4] = {128, (uint64_t)d.q_stride_h * 2, (uint64_t)d.q_stride_t * 2, (uint64_t)d.q_stride_b * 2};
+  const uint64_t q_strides[4] = {128, d.h > 1 ? (uint64_t)d.q_stride_h * 2 : 512,  // of one element: any
+                                 d.queries > 1 ? (uint64_t)d.q_stride_t * 2 : 512, b.batch > 1 ? (uint64_t)d.q_stride_b * 2 : 512};
   const uint32_t q_box[5] = {64, 1, (uint32_t)p.groups, (uint32_t)p.nw, 1};
   // keys [64 elements][entries of a page][64-element blocks][heads][pages]; box: the entries of a page (at most 128)
   const uint64_t k_dims[5] = {64, (uint64_t)c.page, blocks, (uint64_t)c.kv, (uint64_t)c.pages};

@@ -65,6 +65,7 @@ def _attend(capi, **over):
     ("cache", {"d": 96}, "SHAPE"), ("cache", {"dtype": 0}, "DTYPE"), ("cache", {"kv": 0}, "INVALID"),
     ("cache", {"kv": 3}, "SHAPE"), ("cache", {"k_pages": None}, "INVALID"), ("cache", {"v_pages": FAKE + 2}, "ALIGN"),
     ("cache", {"stride_entry": 130}, "ALIGN"), ("cache", {"stride_head": 0}, "INVALID"),
+    ("cache", {"mass": FAKE + 4}, "ALIGN"), ("cache", {"meta_head": 18}, "ALIGN"), ("cache", {"kv": 65536}, "SHAPE"),
     ("batch", {"batch": -1}, "INVALID"), ("batch", {"batch": 65536}, "SHAPE"), ("batch", {"lengths": None}, "INVALID"),
     ("batch", {"block_table": None}, "INVALID"), ("batch", {"width": 1 << 28}, "SHAPE"),
     ("desc", {"h": 130}, "SHAPE"), ("desc", {"h": 0}, "INVALID"), ("desc", {"sinks": -1}, "INVALID"),
@@ -86,7 +87,9 @@ def test_the_other_calls_refuse_on_the_host(capi):
     c, b = _cache(capi), _batch(capi)
     o = capi.PbkPagedObserveDesc(8, 16, 0.1, 0, FAKE, 8192, 1024, 128)
     assert L.pbk_paged_observe(_cache(capi, mass=None), b, o, FAKE, 1 << 40, None) == capi.PBK_ERR_INVALID
-    o.queries = 1025
+    o.q_stride_t = 0
+    assert L.pbk_paged_observe(c, b, o, FAKE, 1 << 40, None) == capi.PBK_ERR_INVALID  # one query's row for all
+    o.queries, o.q_stride_t = 1025, 1024
     assert L.pbk_paged_observe(c, b, o, FAKE, 1 << 40, None) == capi.PBK_ERR_SHAPE
     assert L.pbk_paged_append(c, b, FAKE, FAKE, 256, 128, 4, None, None) == capi.PBK_ERR_INVALID  # 4 tokens, 3 sequences
     assert L.pbk_paged_append(c, b, FAKE, FAKE + 8, 256, 128, 3, None, None) == capi.PBK_ERR_ALIGN
@@ -97,6 +100,7 @@ def test_the_other_calls_refuse_on_the_host(capi):
     assert sel(32, 0, 0, 31) == capi.PBK_ERR_SHAPE        # capacity 80, budget 32: 32 moves
     assert sel(64, 0, 0, 15) == capi.PBK_ERR_SHAPE        # 16 moves
     assert sel(32, 0, 0, 32, _cache(capi, pos=None)) == capi.PBK_ERR_INVALID
+    assert sel(32, 0, 0, 32, c, _batch(capi, width=(1 << 19) + 1)) == capi.PBK_ERR_SHAPE  # over 2^23 entries
     assert sel(32, 0, 0, 32, c, _batch(capi, seen=None)) == capi.PBK_ERR_INVALID
     assert L.pbk_paged_move(c, b, FAKE, None, FAKE, 3, None) == capi.PBK_ERR_INVALID
     none = _batch(capi, batch=0)

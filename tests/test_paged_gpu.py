@@ -559,3 +559,15 @@ def test_refusals(cuda_device):
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
     P.paged_observe_(cache, many[:, :0], table[:1], lens[:1])
     assert _capi.device_error() == 0
+
+
+def test_example_keeps_its_budget_and_agrees_where_nothing_leaves(cuda_device):
+    """The example: with a budget that holds everything the bounded stream is the whole one's (the
+    weights change no result), with a smaller one the cache stays within it plus a page."""
+    from examples.bounded_decode import main
+    common = ["--batch", "2", "--prompt", "90", "--tokens", "20", "--layers", "2", "--hidden", "256", "--heads", "4",
+              "--kv", "2", "--observe", "8", "--recent", "8"]
+    same = main(common + ["--budget", "112"])
+    assert same["bounded"] == same["whole"] == 110 and max(abs(d) for d in same["drift"]) < 1e-5
+    small = main(common + ["--budget", "48"])
+    assert 48 <= small["bounded"] <= 48 + 16
