@@ -23,7 +23,7 @@ namespace {
 constexpr int kUnit = 16;           // entries per unit
 constexpr int kRing = 192 * 1024;   // staging bytes per CTA
 constexpr int kMinUnits = 2;        // units per warp below which fewer warps take part
-constexpr int kClusterUnits = 160;  // most units per CTA where a cluster takes a whole head
+constexpr int kClusterUnits = 320;  // most units per CTA where a cluster takes a whole head
 constexpr int kJoinThreads = 256;
 constexpr int kMassThreads = 256;
 constexpr int kPad = 4;             // floats after a partial row's D values: maximum, sum, two unused
@@ -781,17 +781,46 @@ struct Plan {
   size_t base, open, part, lse2, scores, bytes;
 };
 
-// CTAs per key head where a cluster takes a whole head (one launch, no workspace without
-// weights), 0 where the equal runs and their join are better. The join costs about 6 us at any
-// size; a cluster costs SMs that its size leaves over and, with ragged lengths, the time of the
-// longest sequence, so it is for heads that fit the SMs at once and CTAs that walk at most
-// kClusterUnits units, by the table's capacity. Clusters of more than one CTA are packed by GPC,
-// which leaves an eighth of the SMs over.
-int head_cluster(int64_t heads, int64_t units_per_head, int row_tiles, int sms) {
-  if (row_tiles > 1 || heads > sms) return 0;
-  int c = 1;
-  while (c < 8 && units_per_head > 2 * Shape<128>::kWarps * c && heads * 2 * c <= sms - sms / 8) c *= 2;
-  return units_per_head <= (int64_t)kClusterUnits * c ? c : 0;
+// Clusters of `size` CTAs of this kernel that the current device holds at once (one CTA fills an
+// SM, and the GPCs have different numbers of them), looked up once per device and size.
+int clusters_at_once(int log_size) {
+  static std::atomic<int> cached[64][4] = {};
+  const int size = 1 << log_size, fallback = paged_sm_count() / size - paged_sm_count() / 8 / size;
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fallback;
+  if ((n = cached[dev][log_size].load(std::memory_order_relaxed)) > 0) return n;
+  static std::atomic<uint64_t> done{0};
+  const void* kernel = (const void*)paged_attend_kernel<128, 1, false, true>;
+  if (paged_allow_smem(kernel, kRing + 1024, done) != cudaSuccess) return fallback;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)size), cfg.blockDim = dim3(32 * Shape<128>::kWarps), cfg.dynamicSmemBytes = kRing + 1024;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)size, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return fallback;
+  }
+  cached[dev][log_size].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// log2 of the CTAs per key head where a cluster takes a whole head (one launch, no workspace
+// without weights), -1 where the equal runs and their join are better. The join costs about 6 us at
+// any size; a cluster costs the SMs that its size leaves over and, with ragged lengths, the time
+// of the longest sequence. So it is for heads whose clusters the device holds at once and CTAs
+// that walk at most kClusterUnits units, by the table's capacity (128 heads of 4000 entries, runs
+// and clusters: 51 and 45 us; 96 heads: 42 and 36 us; with lengths spread over 1 .. 4000: 33 and
+// 34, 30 and 33 us). The cluster is the largest that leaves every warp two units. A CTA alone reads
+// some 75 GB/s, so that clusters on few of the SMs fall behind earlier (16 heads of 16000 entries on
+// 64 CTAs: 34 us; the runs take 21 us for lengths spread over 1 .. 16000).
+int head_cluster(int64_t heads, int64_t units_per_head, int row_tiles) {
+  if (row_tiles > 1 || heads > paged_sm_count()) return -1;
+  int c = 0;
+  while (c < 3 && units_per_head > (int64_t)2 * Shape<128>::kWarps << c && heads <= clusters_at_once(c + 1)) ++c;
+  const int most = 5 * (heads << c) >= 3 * paged_sm_count() ? kClusterUnits : kClusterUnits / 2;
+  return units_per_head <= (int64_t)most << c ? c : -1;
 }
 
 Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_attend_desc& d) {
@@ -811,7 +840,8 @@ Plan make_plan(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_pag
   p.units_per_head = per;
   const int64_t heads = (int64_t)b.batch * c.kv, units = per * heads * p.rt;
   const int sms = paged_sm_count();
-  p.cluster = head_cluster(heads, per, p.rt, sms);
+  const int log_cluster = head_cluster(heads, per, p.rt);
+  p.cluster = log_cluster < 0 ? 0 : 1 << log_cluster;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
