@@ -13,10 +13,11 @@
 // Keys are cut into tiles of 128 entries of one (sequence, key head); all tiles stand in one line
 // and each CTA (one per SM) takes an equal run of it. Row tiles hold as many whole queries as fit
 // 128 rows; up to kMaxTiles of them share each key tile, more take further launches. Warps: 0 and
-// 10 TMA producers (a key tile is up to 64 boxes, page by page, and one warp issues a box in
-// about 45 ns; queries come as one box of heads x queries), 1 MMA issuer, 2-5 and 6-9 two groups
-// that take alternate key tiles from four accumulators in TMEM. Every wait is bounded; on timeout
-// the kernel records an error code and winds down.
+// 18 TMA producers (a key tile is up to 64 boxes, page by page, and one warp issues a box in
+// about 45 ns; queries come as one box of heads x queries), 1 MMA issuer, 2-17 four groups that
+// take the key tiles in turn, each from its own accumulator in TMEM (pass 2 over 131072 entries
+// and 8 heads: 66 us with two groups, 60 with four). Every wait is bounded; on timeout the kernel
+// records an error code and winds down.
 //
 // What bounds it: per key tile and pass 128 x 128 exponentials (16 a clock and SM: 0.55 us), the
 // keys' bytes (32 KB at an SM's share of HBM: 0.75 us) and 0.37 us of MMA.
@@ -33,8 +34,9 @@ namespace {
 constexpr int kTile = 128;       // entries of a key tile, rows of a row tile
 constexpr int kMaxTiles = 8;     // row tiles of a launch
 constexpr int kProducers = 2;    // producer warps: warp 0 and the one after the epilogue's
-constexpr int kThreads = 320 + 32 * (kProducers - 1);
-constexpr int kGroup = 128;      // threads of an epilogue group
+constexpr int kGroups = 4;       // epilogue groups of four warps, each with an accumulator in TMEM
+constexpr int kEpilogue = 128 * kGroups;
+constexpr int kThreads = 32 * (kProducers + 1) + kEpilogue;
 constexpr uint32_t kTmemCols = 512;
 
 // Stages of the key and query rings. One row tile (ONE) stays for all of a head's key tiles, and
@@ -131,7 +133,7 @@ __device__ __forceinline__ void landed(uint32_t (&x)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(x[i]));
 }
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory"); }
 
 // A CTA's run of the line of key tiles, one head at a time.
 struct Run {
@@ -170,11 +172,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* keys = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* queries = keys + S::kKeys * S::kBytes;
-  __shared__ uint64_t k_full[S::kKeys], k_empty[S::kKeys], q_full[S::kQueries], q_empty[S::kQueries], s_full[4], s_empty[4],
-      drain;
+  __shared__ uint64_t k_full[S::kKeys], k_empty[S::kKeys], q_full[S::kQueries], q_empty[S::kQueries], s_full[kGroups],
+      s_empty[kGroups], drain;
   constexpr int kRows = ONE ? kTile : kMaxTiles * kTile;
-  // pass 1: the groups' (maximum, sum) per row; of one row tile the second group's, at the end
-  __shared__ float2 s_stat[PASS == 1 && !ONE ? 2 : 1][PASS == 1 ? kRows : 1];
+  // pass 1: the groups' (maximum, sum) per row; of one row tile joined at the end, group by group
+  __shared__ float2 s_stat[PASS == 1 && !ONE ? kGroups : 1][PASS == 1 ? kRows : 1];
   __shared__ __align__(16) float s_lse[PASS == 2 ? kRows : 4];  // pass 2: negated
   __shared__ int s_place[PASS == 2 ? kRows : 1];
   __shared__ int64_t s_sum[kThreads / 32], s_off;
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < S::kKeys; ++s) tc::mbar_init(&k_full[s], 1), tc::mbar_init(&k_empty[s], 1);
     for (int s = 0; s < S::kQueries; ++s) tc::mbar_init(&q_full[s], 1), tc::mbar_init(&q_empty[s], 1);
-    for (int s = 0; s < 4; ++s) tc::mbar_init(&s_full[s], 1), tc::mbar_init(&s_empty[s], kGroup);
+    for (int s = 0; s < kGroups; ++s) tc::mbar_init(&s_full[s], 1), tc::mbar_init(&s_empty[s], 128);
     tc::mbar_init(&drain, 1);
     abort_flag = 0;
     s_seq = -1;
@@ -250,9 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     return true;
   };
 
-  if (warp == 0 || warp >= 10) {
+  if (warp == 0 || warp >= 2 + 4 * kGroups) {
     // ------------------------------------------------------------ TMA producers
-    const int producer = warp == 0 ? 0 : warp - 9;
+    const int producer = warp == 0 ? 0 : warp - 1 - 4 * kGroups;
     const int rows = min(a.page, kTile);  // entries per box
     // this lane's box of every key tile: a page's entries, 64 elements of the head
     const int box = lane * kProducers + producer, at = box / (D / 64) * rows, block = box % (D / 64);
@@ -328,8 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(&k_full[ks], k_phase, 3);
           for (int rt = 0; ok && rt < a.tiles; ++rt) {
             if (!ONE && !(ok = wait(&q_full[qs], q_phase, 4))) break;
-            const uint32_t u = (kt >> 1) * a.tiles + rt, buf = (kt & 1) * 2 + (u & 1);  // the group's u-th product
-            if (u >= 2 && !(ok = wait(&s_empty[buf], ((u >> 1) - 1) & 1, 5))) break;
+            const uint32_t buf = kt % kGroups, u = kt / kGroups * a.tiles + rt;  // the group's u-th product
+            if (u >= 1 && !(ok = wait(&s_empty[buf], (u - 1) & 1, 5))) break;
             tc::fence_after_sync();
             const uint64_t kd0 = k_desc + ks * (S::kBytes >> 4), qd0 = q_desc + qs * (S::kBytes >> 4);
 #pragma unroll
@@ -356,22 +358,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_wait(&drain, 0, 200000000ull);
     }
   } else {
-    // ------------------------------------------------------------ the two epilogue groups
+    // ------------------------------------------------------------ the epilogue groups
     const int group = (warp - 2) >> 2, quad = warp & 3, me = quad * 32 + lane;  // a row (pass 1) or an entry (pass 2)
-    const int et = tid - 64;                                                 // 0 .. 255 over both groups
+    const int et = tid - 64;                                                 // 0 .. kEpilogue - 1
     const int rows = a.tiles * kTile;
     uint32_t kt = 0, used = 0;
     bool ok = true;
     auto take = [&](uint32_t& taddr) -> bool {  // the group's next accumulator
-      const uint32_t buf = group * 2 + (used & 1);
-      if (!__all_sync(0xffffffffu, wait(&s_full[buf], (used >> 1) & 1, 6))) return false;
+      if (!__all_sync(0xffffffffu, wait(&s_full[group], used & 1, 6))) return false;
       tc::fence_after_sync();
-      taddr = tmem + ((uint32_t)(quad * 32) << 16) + buf * kTile;
+      taddr = tmem + ((uint32_t)(quad * 32) << 16) + group * kTile;
       return true;
     };
     auto give = [&]() {
       tc::fence_before_sync();
-      tc::mbar_arrive(&s_empty[group * 2 + (used & 1)]);
+      tc::mbar_arrive(&s_empty[group]);
       ++used;
     };
     // the place in the sequence of row r of the launch: its token's entry; -1 when it has none
@@ -384,14 +385,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 ml = make_float2(-INFINITY, 0.f);  // pass 1, ONE: this thread's row
       if (PASS == 1) {
         if (!ONE)
-          for (int r = et; r < 2 * rows; r += 256) s_stat[r / rows][r % rows] = ml;
+          for (int r = et; r < kGroups * rows; r += kEpilogue) s_stat[r / rows][r % rows] = ml;
         group_sync();
       } else {
         group_sync();  // the last head's logarithms have been read
         // the runs that hold this head, from its first tile in the line
         const int64_t first = from + mine_tiles - run.left - run.t;
         const int run0 = (int)(first / length), run1 = (int)((first + run.tiles - 1) / length);
-        for (int r = et; r < rows; r += 256) {
+        for (int r = et; r < rows; r += kEpilogue) {
           float lse = -INFINITY;
           if (place(r) >= 0) {
             if (run0 == run1) {
@@ -427,9 +428,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = (run.t + i) * kTile + me;
         return e < run.n ? paged::page_of(a.table + run.b * a.table_stride, e, a.log_page, a.pages) : -1;
       };
-      id = page_id((int)(kt & 1) == group ? 0 : 1);
+      id = page_id((int)((group - kt) % kGroups));  // its first tile of this head
       for (int i = 0; ok && i < run.count; ++i, ++kt) {
-        if ((int)(kt & 1) != group) continue;
+        if ((int)(kt % kGroups) != group) continue;
         const int t = (run.t + i), e0 = t * kTile;
         const bool whole = e0 + kTile <= run.n - a.queries + 1;  // every row with a place sees all of the tile
         float* to = nullptr;
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             to = a.mass + id * a.meta_page + run.h * a.meta_head + ((e0 + me) & (a.page - 1));
             have = *to;
           }
-          id = page_id(i + 2);
+          id = page_id(i + kGroups);
         }
         if (PASS == 1) {
           for (int rt = 0; rt < a.tiles; ++rt) {
@@ -447,32 +448,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = take(taddr))) break;
             const int end_col = whole ? kTile : min(kTile, place(rt * kTile + me) + 1 - e0);  // columns the row sees
             if (!ONE) ml = s_stat[group][rt * kTile + me];
-            uint32_t x[4][32];
+            const uint64_t c2 = pack2(a.c, a.c);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {  // 64 columns at a time
+              uint32_t x[2][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tc::tmem_ld_32x32(taddr + 32 * i, x[i]);
+              for (int i = 0; i < 2; ++i) tc::tmem_ld_32x32(taddr + 64 * half + 32 * i, x[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) landed(x[i]);
-            give();
-            if (!whole)
+              for (int i = 0; i < 2; ++i) landed(x[i]);
+              if (half == 1) give();
+              if (!whole)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (32 * i + j >= end_col) x[i][j] = 0xff800000u;  // -inf
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                  for (int j = 0; j < 32; ++j)
+                    if (64 * half + 32 * i + j >= end_col) x[i][j] = 0xff800000u;  // -inf
+              float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
+              for (int j = 0; j < 32; j += 4)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[i][j])), __uint_as_float(x[i][j + 1]));
-            const float up = fmaxf(ml.x, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), mc = finite(up) * a.c;
-            const uint64_t c2 = pack2(a.c, a.c), d2 = pack2(-mc, -mc), d[8] = {d2, d2, d2, d2, d2, d2, d2, d2};
-            uint64_t sum[4] = {0, 0, 0, 0};  // pairs of zeros
+                for (int i = 0; i < 4; ++i)
+                  top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[i & 1][j + (i >> 1)])),
+                                 __uint_as_float(x[i & 1][j + 2 + (i >> 1)]));
+              const float up = fmaxf(ml.x, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), mc = finite(up) * a.c;
+              const uint64_t d2 = pack2(-mc, -mc), d[8] = {d2, d2, d2, d2, d2, d2, d2, d2};
+              uint64_t sum[4] = {0, 0, 0, 0};  // pairs of zeros
 #pragma unroll
-            for (int i = 0; i < 8; ++i) add_exps(sum, x[i / 2] + 16 * (i & 1), c2, d);
-            const float2 part = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-            ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + (part.x + part.y);
-            ml.x = up;
+              for (int i = 0; i < 4; ++i) add_exps(sum, x[i / 2] + 16 * (i & 1), c2, d);
+              const float2 part = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+              ml.y = ml.y * ex2((ml.x - finite(up)) * a.c) + (part.x + part.y);
+              ml.x = up;
+            }
             if (!ONE) s_stat[group][rt * kTile + me] = ml;
           }
         } else {
@@ -482,28 +488,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t taddr;
             if (!(ok = take(taddr))) break;
             const int valid = min(a.nw, a.queries - a.w0 - rt * a.nw) * a.groups;
-            uint32_t x[2][32];  // a chunk of 32 rows is on its way while the one before it is summed
-            tc::tmem_ld_32x32(taddr, x[0]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (32 * i >= valid) break;
-              landed(x[i & 1]);
-              if (i < 3 && 32 * i + 32 < valid) tc::tmem_ld_32x32(taddr + 32 * i + 32, x[(i + 1) & 1]);
+              uint32_t x[32];
+              tc::tmem_ld_32x32(taddr + 32 * i, x);
+              landed(x);
               const ulonglong2* d4 = reinterpret_cast<const ulonglong2*>(s_lse + rt * kTile + 32 * i);
               const int* at = s_place + rt * kTile + 32 * i;
-              const uint32_t(&y)[32] = x[i & 1];
               if (whole && 32 * i + 32 <= valid) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                   uint64_t d[8];
 #pragma unroll
                   for (int k = 0; k < 4; ++k) d[2 * k] = d4[4 * j + k].x, d[2 * k + 1] = d4[4 * j + k].y;
-                  add_exps(sum, y + 16 * j, c2, d);
+                  add_exps(sum, x + 16 * j, c2, d);
                 }
               } else {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                  const float w = ex2(__uint_as_float(y[j]) * a.c + s_lse[rt * kTile + 32 * i + j]);
+                  const float w = ex2(__uint_as_float(x[j]) * a.c + s_lse[rt * kTile + 32 * i + j]);
                   sum[j & 3] = add2(sum[j & 3], pack2(e0 + me <= at[j] ? w : 0.f, 0.f));
                 }
               }
@@ -516,14 +520,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (PASS == 1) {
-        if (ONE && group == 1) s_stat[0][me] = ml;
-        group_sync();
+        if (ONE)
+          for (int i = 0; i < kGroups; ++i) {
+            if (group == i) {
+              const float2 x = i == 0 ? make_float2(-INFINITY, 0.f) : s_stat[0][me];
+              const float up = fmaxf(x.x, ml.x);
+              s_stat[0][me] = make_float2(up, x.y * ex2((x.x - finite(up)) * a.c) + ml.y * ex2((ml.x - finite(up)) * a.c));
+            }
+            group_sync();
+          }
+        else
+          group_sync();
         float2* part = a.part + ((int64_t)blockIdx.x * 2 + (run.t == 0 ? 1 : 0)) * rows;
-        for (int r = ONE ? me : et; r < rows; r += 256) {
-          if (ONE && group == 1) break;
-          const float2 x = ONE ? ml : s_stat[0][r], y = ONE ? s_stat[0][r] : s_stat[ONE ? 0 : 1][r];
-          const float up = fmaxf(x.x, y.x);
-          const float sum = x.y * ex2((x.x - finite(up)) * a.c) + y.y * ex2((y.x - finite(up)) * a.c);
+        for (int r = et; r < rows; r += kEpilogue) {
+          constexpr int kSets = ONE ? 1 : kGroups;
+          float up = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kSets; ++i) up = fmaxf(up, s_stat[i][r].x);
+#pragma unroll
+          for (int i = 0; i < kSets; ++i) sum += s_stat[i][r].y * ex2((s_stat[i][r].x - finite(up)) * a.c);
           if (run.count == run.tiles) a.lse[head * rows + r] = finite(up) * a.c + log2f(sum);
           else part[r] = make_float2(up, sum);
         }
