@@ -886,7 +886,7 @@ cudaError_t launch(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, co
   const bool by_head = query_heads <= p.runs;
   const cudaError_t j = launch_after(paged_join_kernel<D, F16>, dim3((unsigned)(by_head ? query_heads : p.runs)),
                                      dim3(kJoinThreads), 0, st, 1, a, p.runs, by_head);
-  if (j != cudaSuccess || !a.accumulate) return j;
+  if (j != cudaSuccess || !a.accumulate || p.units_per_head == 0) return j;
   const int64_t slices = (p.units_per_head * 4 + kMassThreads - 1) / kMassThreads;
   return launch_after(paged_mass_kernel,
                       dim3((unsigned)((int64_t)a.batch * a.kv), (unsigned)(slices < 65535 ? slices : 65535)),
@@ -936,8 +936,8 @@ cudaError_t launch_paged_attend(const pbk_paged_cache& c, const pbk_paged_batch&
     const uint64_t strides[4] = {any ? (uint64_t)c.stride_entry * 2 : 512, 128, any ? (uint64_t)c.stride_head * 2 : 512,
                                  any ? (uint64_t)c.stride_page * 2 : 512};
     const uint32_t box[5] = {64, (uint32_t)(c.page < kUnit ? c.page : kUnit), (uint32_t)(c.d / 64), 1, 1};
-    const void* k = any ? c.k_pages : ws;
-    const void* v = any ? c.v_pages : ws;
+    const void* k = any ? c.k_pages : d.q;
+    const void* v = any ? c.v_pages : d.q;
     if (!make_tmap_bf16_sw128(&mk, k, 5, dims, strides, box) || !make_tmap_bf16_sw128(&mv, v, 5, dims, strides, box))
       return cudaErrorInvalidValue;
   }

@@ -571,3 +571,23 @@ def test_example_keeps_its_budget_and_agrees_where_nothing_leaves(cuda_device):
     assert same["bounded"] == same["whole"] == 110 and max(abs(d) for d in same["drift"]) < 1e-5
     small = main(common + ["--budget", "48"])
     assert 48 <= small["bounded"] <= 48 + 16
+
+
+@pytest.mark.parametrize("batch", [2, 200])
+def test_a_pool_without_pages_and_a_table_without_columns(cuda_device, batch):
+    """Nothing to read is no error: attention gives zeros, the other calls do nothing."""
+    from pseudobrain_b200 import paged_cache as P
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    q = torch.ones(batch, 4, 64, dtype=torch.bfloat16, device=cuda_device)
+    for pages, width in ((0, 3), (5, 0)):
+        cache = P.PagedCache.allocate(pages, 2, 16, 64, device=cuda_device)
+        table, lens = i32(batch, width), i32(batch) + 40
+        for accumulate in (False, True):
+            out, lse = P.paged_attend(cache, q, table, lens, accumulate=accumulate)
+            assert bool((out == 0).all()) and bool(lse.isneginf().all())
+        P.paged_append_(cache, q[:, :2].contiguous(), q[:, :2].contiguous(), table, lens)
+        P.paged_observe_(cache, q[:, None], table, lens)
+        P.paged_evict_(cache, table, lens, lens, 8)
+        src, dst, count = P.select_evictions(cache, table, lens, lens, 8)
+        assert bool((count == 0).all()) and bool((src == -1).all()) and bool((dst == -1).all())
+        assert bool((cache.mass == 0).all())
