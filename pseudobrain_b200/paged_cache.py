@@ -93,7 +93,7 @@ class PagedCache:
             d.meta_page, d.meta_head = t.stride()[:2]
         d.mass = None if self.mass is None else self.mass.data_ptr()
         d.pos = None if self.pos is None else self.pos.data_ptr()
-        self._ref, self._index = _byref(d), self.device.index
+        self._ref, self._index, self._only_gpu = _byref(d), self.device.index, torch.cuda.device_count() == 1
 
     @classmethod
     def allocate(cls, pages: int, kv: int, page: int, hd: int, dtype: torch.dtype = torch.bfloat16,
@@ -119,11 +119,13 @@ def _call(cache: PagedCache, fn, what: str, *args) -> None:
     serving step makes many small calls, so the common case (that device is current) takes the
     stream's handle without making a Stream object."""
     i = cache._index
-    if torch.cuda.current_device() == i:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(i)), what)
+    if cache._only_gpu or torch.cuda.current_device() == i:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(i)), what)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if status:
+        check(status, what)
 
 
 def _batch(cache: PagedCache, table: torch.Tensor, lengths: torch.Tensor | None, seen: torch.Tensor | None = None):
@@ -173,8 +175,9 @@ def paged_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_tab
     Tokens past the table's capacity are left out."""
     _need(cache, "paged_append_", "k_pages")
     _rows(k, cache, "k")
-    if k.dim() != 3 or k.shape[1] != cache.kv or v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride() \
-            or v.device != k.device:
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 3 or shape[1] != cache._desc.kv or v.shape != shape or v.dtype != k.dtype or v.stride() != strides \
+            or v.get_device() != cache._index:
         raise ValueError(f"paged_append_: k and v must be alike, [N, {cache.kv}, hd], got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
     b = _batch(cache, block_table, lengths, seen)
@@ -182,10 +185,10 @@ def paged_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_tab
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (b.batch + 1,) or not cu_seqlens.is_contiguous() \
                 or cu_seqlens.device != cache.device:
             raise ValueError(f"cu_seqlens must be contiguous int32 [{b.batch + 1}] on the cache's GPU")
-    elif k.shape[0] != b.batch:
-        raise ValueError(f"paged_append_: {k.shape[0]} tokens for {b.batch} sequences need cu_seqlens")
+    elif shape[0] != b.batch:
+        raise ValueError(f"paged_append_: {shape[0]} tokens for {b.batch} sequences need cu_seqlens")
     _call(cache, LIB.pbk_paged_append, "pbk_paged_append", cache._ref, _byref(b), k.data_ptr(), v.data_ptr(),
-          k.stride(0), k.stride(1), k.size(0), None if cu_seqlens is None else cu_seqlens.data_ptr())
+          strides[0], strides[1], shape[0], None if cu_seqlens is None else cu_seqlens.data_ptr())
 
 
 def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -198,26 +201,28 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
     and lse [B, H], the natural logarithm of the sum of exponentials. A sequence without
     entries gives 0 and -inf. ``accumulate`` adds every entry's weight, summed over the query
     heads of its key head, to cache.mass."""
-    _need(cache, "paged_attend", "k_pages", *(("mass",) if accumulate else ()))
+    _need(cache, "paged_attend", "k_pages")
+    if accumulate:
+        _need(cache, "paged_attend", "mass")
     _rows(q, cache, "q")
     b = _batch(cache, block_table, lengths)
-    if q.dim() != 3 or q.shape[0] != b.batch:
+    if q.dim() != 3 or (shape := q.shape)[0] != b.batch:
         raise ValueError(f"paged_attend: q must be [{b.batch}, H, hd], got {tuple(q.shape)}")
     if window is not None and window < 1:
         raise ValueError("paged_attend: the window holds at least the new token (None: no window)")
-    n, h, d = q.shape
+    n, h, d = shape
     sb, sh, _ = q.stride()
     if out is None:
-        out, ob, oh = torch.empty_like(q, memory_format=torch.contiguous_format), h * d, d
-    elif out.shape != q.shape or out.dtype not in (q.dtype, torch.float32) or out.stride(-1) != 1 \
+        out, ob, oh, dtype = torch.empty_like(q, memory_format=torch.contiguous_format), h * d, d, cache._desc.dtype
+    elif out.shape != shape or out.dtype not in (q.dtype, torch.float32) or out.stride(-1) != 1 \
             or out.device != q.device:
-        raise ValueError(f"paged_attend: out must be {tuple(q.shape)}, {q.dtype} or fp32, with a contiguous last dim")
+        raise ValueError(f"paged_attend: out must be {tuple(shape)}, {q.dtype} or fp32, with a contiguous last dim")
     else:
-        ob, oh, _ = out.stride()
-    lse = torch.empty(n, h, dtype=torch.float32, device=q.device)
+        (ob, oh, _), dtype = out.stride(), _DTYPES[out.dtype]
+    lse = torch.empty(n, h, dtype=torch.float32, device=cache.device)
     desc = PbkPagedAttendDesc(h, 0 if window is None else min(window, _INT_MAX), min(sinks, _INT_MAX), accumulate,
-                              d ** -0.5 if scale is None else scale, _DTYPES[out.dtype], q.data_ptr(), sb, sh, out.data_ptr(), ob,
-                              oh, lse.data_ptr())
+                              d ** -0.5 if scale is None else scale, dtype, q.data_ptr(), sb, sh, out.data_ptr(), ob, oh,
+                              lse.data_ptr())
     bref, dref = _byref(b), _byref(desc)
     _run(cache, LIB.pbk_paged_attend, "pbk_paged_attend", LIB.pbk_paged_attend_workspace(cache._ref, bref, dref),
          cache._ref, bref, dref)

@@ -1,12 +1,14 @@
 """GPU parity of the paged cache's operators against their definitions in float64
 (oracle/paged.py).
 
-Tolerances, from the number formats (u = unit roundoff: 2^-9 for bf16, 2^-11 for fp16 with a
-significand bit to spare each): a weight p enters the product with the values in 16 bits
-(error u p) and the result is rounded once (u |out|, none in fp32). Scores are fp32 sums of
-exact 16-bit products: with sum |q k| scale <= 64 and at most 16 chained additions their error
-is below 64 * 16 * 2^-23 = 1.3e-4, which is also the relative error of a weight and, with the
-sum of exponentials, the absolute one of the logarithm: SCORE = 2^-12 covers both.
+Tolerances, from the number formats: the result is rounded once to its type, by at most 2^-8 of
+it in bf16, 2^-11 in fp16 and nothing in fp32, and a weight enters the product with the values
+as one fp16 number (2^-11 of it) or as two bf16 numbers (less than 2^-16): u_p + u_out with
+u = 2^-9 for bf16 and 2^-11 for fp16 covers both, and what one bf16 number per weight would lose
+(2^-8) it does not. Scores are fp32 sums of exact 16-bit products: with sum |q k| scale <= 64
+and at most 16 chained additions their error is below 64 * 16 * 2^-23 = 1.3e-4, which is also
+the relative error of a weight and, with the sum of exponentials, the absolute one of the
+logarithm: SCORE = 2^-12 covers both.
     |out - ref| <= (u_p + u_out + SCORE) sum p |v|,  |lse - ref| <= SCORE,
     |mass - ref| <= 2 SCORE * weight + 2^-22 mass.
 Everything else (append, select, move) is exact.
