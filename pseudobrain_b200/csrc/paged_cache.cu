@@ -136,8 +136,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(x));
   return x;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 // A word (four words) of CTA `rank`'s shared memory, at the place that `p` has in this CTA's.
 __device__ __forceinline__ uint32_t remote_at(const uint32_t* p, uint32_t rank) {
@@ -360,22 +363,34 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
   const uint32_t done = __reduce_add_sync(0xffffffffu, theirs);
   uint32_t hole_run = __reduce_add_sync(0xffffffffu, lane < (int)rank ? theirs : 0u);
   uint32_t move_run = __reduce_add_sync(0xffffffffu, lane < (int)rank ? moved : 0u);
-  cluster_sync();  // no CTA leaves while another reads its counts
+  cluster_arrive();  // this CTA has read the others' shared memory for the last time
+  uint32_t* ranks = hist;  // of a turn's words: the places their entries take in dst and src
   for (int turn = 0; turn < turns; ++turn) {
-    const int w = turn * THREADS + tid;
-    uint32_t hole = 0, mover = 0, total;
+    const int first = turn * THREADS, w = first + tid, left = min(w1 - w0 - first, THREADS);
+    uint32_t hole = 0, mover = 0, all_h, all_m;
     if (w < w1 - w0) hole = masks[2 * w], mover = masks[2 * w + 1];
-    uint32_t at = hole_run + cta_prefix<THREADS>((uint32_t)__popc(hole), scratch, &total);
-    hole_run += total;
+    uint32_t hole_at = hole_run + cta_prefix<THREADS>((uint32_t)__popc(hole), scratch, &all_h);
     __syncthreads();
-    for (; hole != 0; hole &= hole - 1u) odst[at++] = e0 + 32 * w + __ffs(hole) - 1;
-    at = move_run + cta_prefix<THREADS>((uint32_t)__popc(mover), scratch, &total);
-    move_run += total;
+    uint32_t move_at = move_run + cta_prefix<THREADS>((uint32_t)__popc(mover), scratch, &all_m);
+    hole_run += all_h, move_run += all_m;
+    if (all_h + all_m <= 2u * left) {  // few: each thread writes its word's
+      for (; hole != 0; hole &= hole - 1u) odst[hole_at++] = e0 + 32 * w + __ffs(hole) - 1;
+      for (; mover != 0; mover &= mover - 1u) osrc[move_at++] = e0 + 32 * w + __ffs(mover) - 1;
+    } else {  // many: the words dealt to the warps, a lane per bit, so that neighbours write neighbours
+      ranks[2 * tid] = hole_at, ranks[2 * tid + 1] = move_at;
+      __syncthreads();
+      for (int j = tid >> 5; j < left; j += THREADS / 32) {
+        const uint32_t hw = masks[2 * (first + j)], mw = masks[2 * (first + j) + 1], below = (1u << lane) - 1u;
+        const int e = e0 + 32 * (first + j) + lane;
+        if (hw >> lane & 1u) odst[ranks[2 * j] + __popc(hw & below)] = e;
+        if (mw >> lane & 1u) osrc[ranks[2 * j + 1] + __popc(mw & below)] = e;
+      }
+    }
     __syncthreads();
-    for (; mover != 0; mover &= mover - 1u) osrc[at++] = e0 + 32 * w + __ffs(mover) - 1;
   }
   if (rank == 0 && tid == 0) count[pair] = (int)done;
   for (int i = (int)done + rank * THREADS + tid; i < moves; i += ctas * THREADS) osrc[i] = odst[i] = -1;
+  cluster_wait();  // no CTA leaves while another may read its shared memory
 }
 
 }  // namespace
