@@ -223,63 +223,74 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
     k.w = i + 3 < mine ? select_key(m.w, p.w, sinks, first_recent) : 0u;
     return k;
   };
+  uint32_t prefix = 0, need = (uint32_t)budget;  // the digits so far; how many of the keys that match them stay
+  // Counts a thread's four keys from entry i on (past the share: none) by the digit at `shift`,
+  // where they match the digits above it. All lanes of a warp call it together.
+  auto count_keys = [&](uint32_t* hst, int shift, int bits, uint4 k, int i) {
+    const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
+    uint32_t bin[4];
+    bool take[4], all = true, any = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bin[j] = (kk[j] >> shift) & ((1u << bits) - 1u);
+      take[j] = i + j < mine && (shift == 21 || (kk[j] ^ prefix) >> (shift + bits) == 0);
+      all = all && take[j] && bin[j] == bin[0];
+      any = any || take[j];
+    }
+    if (!__any_sync(0xffffffffu, any)) return;
+    // many entries may share a key (protected ones, those without weight yet): a warp whose 128
+    // agree counts them at once
+    const uint32_t first = __shfl_sync(0xffffffffu, bin[0], 0);
+    if (__all_sync(0xffffffffu, all && bin[0] == first)) {
+      if (lane == 0) atomicAdd(&hst[bin[0]], 128u);
+    } else if (all) {
+      atomicAdd(&hst[bin[0]], 4u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (take[j]) atomicAdd(&hst[bin[j]], 1u);
+    }
+  };
+
   for (int i = tid; i < (ctas > 1 ? 6 : 3) * kBins; i += THREADS) hist[i] = 0;  // and the sums
+  if (ctas > 1) cluster_arrive();  // (waited for before anyone adds to another's sums)
+  __syncthreads();
   if (KEEP) {
-    // all of a thread's loads of a turn are in flight together
+    // the keys into shared memory, the first digit counted on the way; all of a thread's loads of
+    // a turn are in flight together
     constexpr int kEach = 4;
-    for (int i0 = 4 * tid; i0 < mine; i0 += 4 * kEach * THREADS) {
+    for (int base = 0; base < mine; base += 4 * kEach * THREADS) {
       uint4 k[kEach];
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) k[j] = load_keys(min(i0 + 4 * j * THREADS, (mine - 1) & ~3));
+      for (int j = 0; j < kEach; ++j) k[j] = load_keys(min(base + 4 * (j * THREADS + tid), (mine - 1) & ~3));
 #pragma unroll
-      for (int j = 0; j < kEach; ++j)
-        if (i0 + 4 * j * THREADS < mine) *reinterpret_cast<uint4*>(keys + i0 + 4 * j * THREADS) = k[j];
+      for (int j = 0; j < kEach; ++j) {
+        const int i = base + 4 * (j * THREADS + tid);
+        if (i < mine) *reinterpret_cast<uint4*>(keys + i) = k[j];
+        count_keys(hist, 21, 11, k[j], i);
+      }
     }
   }
-  if (ctas > 1) cluster_sync();  // the sums are zero before anyone adds to them
-  else __syncthreads();
-  uint32_t prefix = 0, need = (uint32_t)budget;  // the digits so far; how many of the keys that match them stay
 #pragma unroll 1
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
     uint32_t* hst = hist + digit * kBins;
-    const uint32_t above = digit == 0 ? 0u : prefix >> (shift + bits);
-    for (int i0 = 0; i0 < mine; i0 += 4 * THREADS) {
-      const int i = i0 + 4 * tid;
-      uint4 k = make_uint4(0u, 0u, 0u, 0u);
-      if (i < mine) {
-        if (KEEP) k = *reinterpret_cast<const uint4*>(keys + i);
-        else k = load_keys(i);
+    if (!KEEP || digit > 0)
+      for (int base = 0; base < mine; base += 4 * THREADS) {
+        const int i = base + 4 * tid;
+        uint4 k = make_uint4(0u, 0u, 0u, 0u);
+        if (i < mine) {
+          if (KEEP) k = *reinterpret_cast<const uint4*>(keys + i);
+          else k = load_keys(i);
+        }
+        count_keys(hst, shift, bits, k, i);
       }
-      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
-      uint32_t bin[4];
-      bool take[4], all = true, any = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bin[j] = (kk[j] >> shift) & ((1u << bits) - 1u);
-        take[j] = i + j < mine && (digit == 0 || (kk[j] >> (shift + bits)) == above);
-        all = all && take[j] && bin[j] == bin[0];
-        any = any || take[j];
-      }
-      if (!__any_sync(0xffffffffu, any)) continue;
-      // many entries may share a key (protected ones, those without weight yet): a warp whose 128
-      // agree counts them at once
-      const uint32_t first = __shfl_sync(0xffffffffu, bin[0], 0);
-      if (__all_sync(0xffffffffu, all && bin[0] == first)) {
-        if (lane == 0) atomicAdd(&hst[bin[0]], 128u);
-      } else if (all) {
-        atomicAdd(&hst[bin[0]], 4u);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (take[j]) atomicAdd(&hst[bin[j]], 1u);
-      }
-    }
     __syncthreads();
     // the cluster's sums: bin i is kept by CTA i / (kBins / ctas)
     const int part = kBins / ctas, log_ctas = 31 - __clz(ctas);
     uint32_t* sum_of = sums + digit * kBins;
     if (ctas > 1) {
+      if (digit == 0) cluster_wait();  // every CTA's sums are zero
       for (int i = tid; i < kBins; i += THREADS)
         if (hst[i] != 0) remote_add(sum_of + (i & (part - 1)), i >> (11 - log_ctas), hst[i]);
       cluster_sync();
