@@ -173,40 +173,49 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, int64_t at, float
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
 }
 
-// Adds the weights of quarter i (four entries; i / 4 counts the head's units) of one (sequence,
-// key head) to their mass: one page id, one 16-byte access to the mass and one to each row's
-// scores serve them. `scores` are those of the head's first unit in the first row tile, `tile`
-// floats from one row tile's to the next's; lse2[r] the rows' logarithms (INFINITY for a row
-// without weight: it adds 0).
-__device__ __forceinline__ void add_weights(const AttendArgs& a, int b, int h, const Span& s, int i,
-                                            const float* scores, int64_t tile, const float* lse2) {
-  const int e = s.entry(i / 4) + i % 4 * 4;
-  if (e >= s.n) return;
-  const int page = a.table[b * a.table_stride + (e >> a.log_page)];
-  const float* x = scores + (int64_t)(i / 4) * (kUnit * a.rows) + i % 4 * 4;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int r0 = 0; r0 < a.groups; r0 += a.rows, x += tile) {
-    const int rows = min(a.rows, a.groups - r0);
+// The mass of quarter i (four entries; i / 4 counts the head's units) of one (sequence, key
+// head): one page id and one 16-byte access serve the four. Loaded apart from the addition, so
+// that it is on its way while the rows' logarithms are still being joined.
+struct Quarter {
+  float4* to = nullptr;  // nullptr: past the length, or on a page outside the pool
+  float4 have;
+  int left;              // entries of the sequence from the quarter's first on
+  __device__ Quarter() {}
+  __device__ Quarter(const AttendArgs& a, int b, int h, const Span& s, int i) {
+    const int e = s.entry(i / 4) + i % 4 * 4;
+    left = s.n - e;
+    if (left <= 0) return;
+    const int page = paged::page_of(a.table + b * a.table_stride, e, a.log_page, a.pages);
+    if (page < 0) return;
+    to = reinterpret_cast<float4*>(a.mass + page * a.meta_page + h * a.meta_head + (e & (a.page - 1)));
+    have = *to;
+  }
+  // Adds the quarter's weights. `scores` are those of the head's first unit in the first row tile,
+  // `tile` floats from one row tile's to the next's; lse2[r] the rows' logarithms (INFINITY for a
+  // row without weight: it adds 0).
+  __device__ void add(const AttendArgs& a, int i, const float* scores, int64_t tile, const float* lse2) const {
+    if (to == nullptr) return;
+    const float* x = scores + (int64_t)(i / 4) * (kUnit * a.rows) + i % 4 * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r0 = 0; r0 < a.groups; r0 += a.rows, x += tile) {
+      const int rows = min(a.rows, a.groups - r0);
 #pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      const float4 y = *reinterpret_cast<const float4*>(x + r * kUnit);
-      const float l = lse2[r0 + r];
-      sum.x += ex2(y.x - l), sum.y += ex2(y.y - l), sum.z += ex2(y.z - l), sum.w += ex2(y.w - l);
+      for (int r = 0; r < rows; ++r) {
+        const float4 y = *reinterpret_cast<const float4*>(x + r * kUnit);
+        const float l = lse2[r0 + r];
+        sum.x += ex2(y.x - l), sum.y += ex2(y.y - l), sum.z += ex2(y.z - l), sum.w += ex2(y.w - l);
+      }
+    }
+    if (left >= 4) {
+      *to = make_float4(have.x + sum.x, have.y + sum.y, have.z + sum.z, have.w + sum.w);
+    } else {  // the sequence's last entries; rows past them are left alone
+      float* f = reinterpret_cast<float*>(to);
+      f[0] = have.x + sum.x;
+      if (left > 1) f[1] = have.y + sum.y;
+      if (left > 2) f[2] = have.z + sum.z;
     }
   }
-  if ((unsigned)page >= (unsigned)a.pages) return;
-  float4* to = reinterpret_cast<float4*>(a.mass + page * a.meta_page + h * a.meta_head + (e & (a.page - 1)));
-  if (e + 4 <= s.n) {
-    float4 y = *to;
-    y.x += sum.x, y.y += sum.y, y.z += sum.z, y.w += sum.w;
-    *to = y;
-  } else {  // the sequence's last entries; rows past them are left alone
-    float* f = reinterpret_cast<float*>(to);
-    f[0] += sum.x;
-    if (e + 1 < s.n) f[1] += sum.y;
-    if (e + 2 < s.n) f[2] += sum.z;
-  }
-}
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
@@ -620,8 +629,17 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     for (int w = 0; w < S::kWarps; ++w) sum += s_ml[w][tid].y * ex2(s_ml[w][tid].x - finite(top));
     s_joined[tid] = make_float2(top, sum);
   }
-  cluster_sync();
+  // this CTA's warps wrote the scores of its own units; its threads add their weights
   const int h = c.pair;
+  int first_quarter = 0, end_quarter = 0;
+  Quarter quarter;
+  if (a.accumulate) {
+    const int parts = ctas * S::kWarps;
+    first_quarter = 4 * (int)((int64_t)c.s.units * (rank * S::kWarps) / parts) + tid;
+    end_quarter = 4 * (int)((int64_t)c.s.units * ((rank + 1) * S::kWarps) / parts);
+    if (first_quarter < end_quarter) quarter = Quarter(a, c.b, h, c.s, first_quarter);
+  }
+  cluster_sync();
   for (int i = rank * kThreads + tid; i < rows * D; i += ctas * kThreads) {
     const int row = i / D, d = i % D;
     float top = -INFINITY, sum = 0.f, y = 0.f;
@@ -643,11 +661,11 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   }
   cluster_sync();  // no CTA leaves while another reads its part
   if (!a.accumulate) return;
-  // this CTA's warps wrote the scores of its own units
-  const int t0 = (int)((int64_t)c.s.units * (rank * S::kWarps) / (ctas * S::kWarps));
-  const int t1 = (int)((int64_t)c.s.units * ((rank + 1) * S::kWarps) / (ctas * S::kWarps));
-  for (int i = 4 * t0 + tid; i < 4 * t1; i += kThreads)
-    add_weights(a, c.b, h, c.s, i, a.scores + (blockIdx.x / ctas) * a.whole_units * (kUnit * a.rows), 0, s_lse);
+  const float* scores = a.scores + (blockIdx.x / ctas) * a.whole_units * (kUnit * a.rows);
+  for (int i = first_quarter; i < end_quarter; i += kThreads) {
+    quarter.add(a, i, scores, 0, s_lse);
+    if (i + kThreads < end_quarter) quarter = Quarter(a, c.b, h, c.s, i + kThreads);
+  }
 }
 
 // Joins the heads that no run held whole: the warps of a block share a head's rows and each
@@ -761,15 +779,20 @@ __global__ void __launch_bounds__(kMassThreads, 6)
   paged::wait_previous();
   const int tid = threadIdx.x, h = blockIdx.x % a.kv, b = blockIdx.x / a.kv;
   const Span s(a, b);
+  int i = blockIdx.y * kMassThreads + tid;
   if (blockIdx.y * kMassThreads >= 4 * s.units) return;
+  Quarter quarter;
+  if (i < 4 * s.units) quarter = Quarter(a, b, h, s, i);
   const int64_t unit = a.base[b] * (a.kv * a.rt) + (int64_t)h * a.rt * s.units;
   if (tid < a.groups) {
     const float x = a.lse2[((int64_t)b * a.kv + h) * a.groups + tid];
     s_lse[tid] = x == -INFINITY ? INFINITY : x;
   }
   __syncthreads();
-  for (int i = blockIdx.y * kMassThreads + tid; i < 4 * s.units; i += gridDim.y * kMassThreads)
-    add_weights(a, b, h, s, i, a.scores + unit * (kUnit * a.rows), (int64_t)s.units * (kUnit * a.rows), s_lse);
+  while (i < 4 * s.units) {
+    quarter.add(a, i, a.scores + unit * (kUnit * a.rows), (int64_t)s.units * (kUnit * a.rows), s_lse);
+    if ((i += gridDim.y * kMassThreads) < 4 * s.units) quarter = Quarter(a, b, h, s, i);
+  }
 }
 
 constexpr size_t align256(size_t x) { return (x + 255) / 256 * 256; }
