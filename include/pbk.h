@@ -742,10 +742,9 @@ PBK_API int pbk_paged_observe(const pbk_paged_cache* cache, const pbk_paged_batc
  * least min(budget, capacity - budget) (capacity = width * page; less is PBK_ERR_SHAPE); places
  * past count hold -1. A row of the table holds at most 2^23 entries. After the moves the sequence has `budget` entries, in no particular
  * order. sinks + recent <= budget. */
-PBK_API size_t pbk_paged_select_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget);
 PBK_API int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget,
                              int32_t recent, int32_t sinks, int32_t* src, int32_t* dst, int32_t* count, int32_t moves,
-                             void* workspace, size_t workspace_bytes, void* stream);
+                             void* stream);
 
 /* Entry dst[b][h][n] := entry src[b][h][n] (key, value, and mass and pos where the cache has
  * them) for n < count[b][h]. The places named by dst must not be sources. Entries outside the

@@ -229,8 +229,7 @@ SIGNATURES = {
     "pbk_paged_attend": (ctypes.c_int, [_PC, _PB, ctypes.POINTER(PbkPagedAttendDesc), _VP, ctypes.c_size_t, _VP]),
     "pbk_paged_observe_workspace": (ctypes.c_size_t, [_PC, _PB, ctypes.POINTER(PbkPagedObserveDesc)]),
     "pbk_paged_observe": (ctypes.c_int, [_PC, _PB, ctypes.POINTER(PbkPagedObserveDesc), _VP, ctypes.c_size_t, _VP]),
-    "pbk_paged_select_workspace": (ctypes.c_size_t, [_PC, _PB, _I32]),
-    "pbk_paged_select": (ctypes.c_int, [_PC, _PB, _I32, _I32, _I32, _VP, _VP, _VP, _I32, _VP, ctypes.c_size_t, _VP]),
+    "pbk_paged_select": (ctypes.c_int, [_PC, _PB, _I32, _I32, _I32, _VP, _VP, _VP, _I32, _VP]),
     "pbk_paged_move": (ctypes.c_int, [_PC, _PB, _VP, _VP, _VP, _I32, _VP]),
     "pbk_ipc_handle": (ctypes.c_int, [_VP, _VP, ctypes.POINTER(ctypes.c_int64)]),
     "pbk_ipc_open": (ctypes.c_int, [_VP, ctypes.POINTER(ctypes.c_void_p)]),

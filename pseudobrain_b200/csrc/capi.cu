@@ -896,14 +896,8 @@ int pbk_paged_observe(const pbk_paged_cache* cache, const pbk_paged_batch* batch
   return launch_status(pbk::launch_paged_observe(*cache, *batch, *desc, workspace, static_cast<cudaStream_t>(stream)));
 }
 
-size_t pbk_paged_select_workspace(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget) {
-  if (validate_paged(cache, batch, 12) != PBK_OK || batch->batch == 0 || budget < 1) return 0;
-  return pbk::paged_select_workspace(*cache, *batch, budget);
-}
-
 int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch, int32_t budget, int32_t recent,
-                     int32_t sinks, int32_t* src, int32_t* dst, int32_t* count, int32_t moves, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     int32_t sinks, int32_t* src, int32_t* dst, int32_t* count, int32_t moves, void* stream) {
   int st = validate_paged(cache, batch, 12);
   if (st != PBK_OK) return st;
   if (budget < 1 || recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget || moves < 0) return PBK_ERR_INVALID;
@@ -912,10 +906,8 @@ int pbk_paged_select(const pbk_paged_cache* cache, const pbk_paged_batch* batch,
   const int64_t past = (int64_t)batch->width * cache->page - budget;
   if (moves < (past < budget ? past : budget)) return PBK_ERR_SHAPE;
   if (!batch->seen || !count || (moves > 0 && (!src || !dst))) return PBK_ERR_INVALID;
-  st = check_workspace(workspace, workspace_bytes, pbk::paged_select_workspace(*cache, *batch, budget));
-  if (st != PBK_OK) return st;
   if ((st = check_current_device()) != PBK_OK) return st;
-  return launch_status(pbk::launch_paged_select(*cache, *batch, budget, recent, sinks, src, dst, count, moves, workspace,
+  return launch_status(pbk::launch_paged_select(*cache, *batch, budget, recent, sinks, src, dst, count, moves,
                                                 static_cast<cudaStream_t>(stream)));
 }
 

@@ -94,9 +94,8 @@ cudaError_t launch_paged_attend(const pbk_paged_cache& c, const pbk_paged_batch&
 size_t paged_observe_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d);
 cudaError_t launch_paged_observe(const pbk_paged_cache& c, const pbk_paged_batch& b, const pbk_paged_observe_desc& d,
                                  void* ws, cudaStream_t st);
-size_t paged_select_workspace(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget);
 cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
-                                int32_t* src, int32_t* dst, int32_t* count, int moves, void* ws, cudaStream_t st);
+                                int32_t* src, int32_t* dst, int32_t* count, int moves, cudaStream_t st);
 cudaError_t launch_paged_move(const pbk_paged_cache& c, const pbk_paged_batch& b, const int32_t* src,
                               const int32_t* dst, const int32_t* count, int moves, cudaStream_t st);
 

@@ -416,10 +416,8 @@ cudaError_t launch_paged_append(const pbk_paged_cache& c, const pbk_paged_batch&
                       cu_seqlens, paged_log2(c.page));
 }
 
-size_t paged_select_workspace(const pbk_paged_cache&, const pbk_paged_batch&, int) { return 0; }
-
 cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch& b, int budget, int recent, int sinks,
-                                int32_t* src, int32_t* dst, int32_t* count, int moves, void*, cudaStream_t st) {
+                                int32_t* src, int32_t* dst, int32_t* count, int moves, cudaStream_t st) {
   // CTAs per (sequence, key head): more while a share holds over 2048 entries and the grid has
   // room on the SMs, and as many as it takes to keep the shares in shared memory
   const int64_t pairs = (int64_t)b.batch * c.kv, cap = (int64_t)b.width * c.page;

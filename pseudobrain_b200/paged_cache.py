@@ -264,9 +264,8 @@ def select_evictions(cache: PagedCache, block_table: torch.Tensor, lengths: torc
     places = torch.empty(2, b.batch, cache.kv, moves, dtype=torch.int32, device=cache.device)
     src, dst = places.unbind(0)
     count = torch.empty(b.batch, cache.kv, dtype=torch.int32, device=cache.device)
-    bref = _byref(b)
-    _run(cache, LIB.pbk_paged_select, "pbk_paged_select", LIB.pbk_paged_select_workspace(cache._ref, bref, budget),
-         cache._ref, bref, budget, recent, sinks, src.data_ptr(), dst.data_ptr(), count.data_ptr(), moves)
+    _call(cache, LIB.pbk_paged_select, "pbk_paged_select", cache._ref, _byref(b), budget, recent, sinks, src.data_ptr(),
+          dst.data_ptr(), count.data_ptr(), moves)
     return src, dst, count
 
 

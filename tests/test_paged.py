@@ -94,7 +94,7 @@ def test_the_other_calls_refuse_on_the_host(capi):
     assert L.pbk_paged_append(c, b, FAKE, FAKE, 256, 128, 4, None, None) == capi.PBK_ERR_INVALID  # 4 tokens, 3 sequences
     assert L.pbk_paged_append(c, b, FAKE, FAKE + 8, 256, 128, 3, None, None) == capi.PBK_ERR_ALIGN
     sel = lambda budget, recent, sinks, moves, cc=c, bb=b: L.pbk_paged_select(  # noqa: E731
-        cc, bb, budget, recent, sinks, FAKE, FAKE, FAKE, moves, FAKE, 1 << 40, None)
+        cc, bb, budget, recent, sinks, FAKE, FAKE, FAKE, moves, None)
     assert sel(32, 30, 3, 32) == capi.PBK_ERR_INVALID     # more protected than kept
     assert sel(0, 0, 0, 32) == capi.PBK_ERR_INVALID
     assert sel(32, 0, 0, 31) == capi.PBK_ERR_SHAPE        # capacity 80, budget 32: 32 moves
