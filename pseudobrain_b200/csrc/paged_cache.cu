@@ -110,7 +110,11 @@ __device__ __forceinline__ uint32_t select_key(float mass, int pos, int sinks, i
 }
 
 constexpr int kBins = 2048;          // a digit of 11 bits
-constexpr int kMostKeys = 32768;     // keys that a CTA keeps in shared memory
+// Keys that a CTA keeps in shared memory. With the masks and the histogram 24576 of them are 110 KB,
+// so that two CTAs share an SM. Against 32768, one CTA per SM (GPU time, sequences x key heads x
+// entries): 60 x 8 x 54806 takes 190 us for 234, 23 x 16 x 198858 756 for 763, but 7 x 16 x 102203
+// 53.5 for 50.7. At 23040 heads of 23742 entries are split: 37 x 16 of them take 76 us for 58.
+constexpr int kMostKeys = 24576;
 constexpr int kMaxCluster = 16;
 
 // Exclusive prefix of x over the CTA's THREADS threads; the sum in *total. Two uses of `scratch`
@@ -184,9 +188,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
     paged_select_kernel(const pbk_paged_cache c, const pbk_paged_batch b, int budget, int recent, int sinks,
                         int32_t* src, int32_t* dst, int32_t* count, int moves, int log_page, int ctas, int share) {
   extern __shared__ __align__(16) uint32_t smem[];
-  uint32_t* hist = smem;                            // [3][kBins] of this CTA's entries
-  uint32_t* sums = hist + 3 * kBins;                // [3][kBins] the cluster's, of this CTA's bins; not for one CTA
-  uint32_t* masks = sums + (ctas > 1 ? 3 * kBins : 0);  // [share / 32][2]
+  uint32_t* hist = smem;                            // [kBins] of this CTA's entries, a digit at a time
+  uint32_t* sums = hist + kBins;                    // [3][kBins / ctas] the cluster's, of this CTA's bins; not for one CTA
+  uint32_t* masks = sums + (ctas > 1 ? 3 * (kBins / ctas) : 0);  // [share / 32][2]
   uint32_t* keys = masks + share / 16;              // [share], 16-byte aligned: share is a multiple of 64
   __shared__ uint32_t scratch[THREADS / 32], found[2], counts[2];
   paged::launch_next();
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
   uint32_t prefix = 0, need = (uint32_t)budget;  // the digits so far; how many of the keys that match them stay
   // Counts a thread's four keys from entry i on (past the share: none) by the digit at `shift`,
   // where they match the digits above it. All lanes of a warp call it together.
-  auto count_keys = [&](uint32_t* hst, int shift, int bits, uint4 k, int i) {
+  auto count_keys = [&](int shift, int bits, uint4 k, int i) {
     const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
     uint32_t bin[4];
     bool take[4], all = true, any = false;
@@ -242,17 +246,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
     // agree counts them at once
     const uint32_t first = __shfl_sync(0xffffffffu, bin[0], 0);
     if (__all_sync(0xffffffffu, all && bin[0] == first)) {
-      if (lane == 0) atomicAdd(&hst[bin[0]], 128u);
+      if (lane == 0) atomicAdd(&hist[bin[0]], 128u);
     } else if (all) {
-      atomicAdd(&hst[bin[0]], 4u);
+      atomicAdd(&hist[bin[0]], 4u);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (take[j]) atomicAdd(&hst[bin[j]], 1u);
+        if (take[j]) atomicAdd(&hist[bin[j]], 1u);
     }
   };
 
-  for (int i = tid; i < (ctas > 1 ? 6 : 3) * kBins; i += THREADS) hist[i] = 0;  // and the sums
+  for (int i = tid; i < kBins + (ctas > 1 ? 3 * (kBins / ctas) : 0); i += THREADS) hist[i] = 0;  // and the sums
   if (ctas > 1) cluster_arrive();  // (waited for before anyone adds to another's sums)
   __syncthreads();
   if (KEEP) {
@@ -267,14 +271,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
       for (int j = 0; j < kEach; ++j) {
         const int i = base + 4 * (j * THREADS + tid);
         if (i < mine) *reinterpret_cast<uint4*>(keys + i) = k[j];
-        count_keys(hist, 21, 11, k[j], i);
+        count_keys(21, 11, k[j], i);
       }
     }
   }
 #pragma unroll 1
   for (int digit = 0; digit < 3; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
-    uint32_t* hst = hist + digit * kBins;
     if (!KEEP || digit > 0)
       for (int base = 0; base < mine; base += 4 * THREADS) {
         const int i = base + 4 * tid;
@@ -283,16 +286,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
           if (KEEP) k = *reinterpret_cast<const uint4*>(keys + i);
           else k = load_keys(i);
         }
-        count_keys(hst, shift, bits, k, i);
+        count_keys(shift, bits, k, i);
       }
     __syncthreads();
     // the cluster's sums: bin i is kept by CTA i / (kBins / ctas)
     const int part = kBins / ctas, log_ctas = 31 - __clz(ctas);
-    uint32_t* sum_of = sums + digit * kBins;
+    uint32_t* sum_of = sums + digit * part;
     if (ctas > 1) {
       if (digit == 0) cluster_wait();  // every CTA's sums are zero
       for (int i = tid; i < kBins; i += THREADS)
-        if (hst[i] != 0) remote_add(sum_of + (i & (part - 1)), i >> (11 - log_ctas), hst[i]);
+        if (hist[i] != 0) remote_add(sum_of + (i & (part - 1)), i >> (11 - log_ctas), hist[i]);
       cluster_sync();
     }
     // bins from the top, kBins / THREADS per thread; the thread whose bins reach `need` tells
@@ -302,11 +305,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
 #pragma unroll
     for (int j = 0; j < kPer; j += 4) {
       const int at = low + kPer - 4 - j;
-      const uint4 x = ctas == 1 ? *reinterpret_cast<const uint4*>(hst + at) : remote4(sum_of + (at & (part - 1)), owner);
+      const uint4 x = ctas == 1 ? *reinterpret_cast<const uint4*>(hist + at) : remote4(sum_of + (at & (part - 1)), owner);
       bins[j] = x.w, bins[j + 1] = x.z, bins[j + 2] = x.y, bins[j + 3] = x.x;
       sum += (x.x + x.y) + (x.z + x.w);
     }
     uint32_t before = cta_prefix<THREADS>(sum, scratch, &total);
+    if (digit < 2)  // (the last digit's counts are read once more below)
+      for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
     if (before < need && before + sum >= need) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 2)
   }
   // prefix is the budget-th key; `need` of the entries equal to it stay, the lowest first
   const uint32_t equal_before =
-      __reduce_add_sync(0xffffffffu, lane < (int)rank ? remote(hist + 2 * kBins + (prefix & 1023u), lane) : 0u);
+      __reduce_add_sync(0xffffffffu, lane < (int)rank ? remote(hist + (prefix & 1023u), lane) : 0u);
   for (int w = tid >> 5; w < w1 - w0; w += (THREADS / 32)) {
     const int i = 32 * w + lane;
     uint32_t k = 0;
@@ -426,7 +431,7 @@ cudaError_t launch_paged_select(const pbk_paged_cache& c, const pbk_paged_batch&
     ctas *= 2;
   const int64_t words = (cap + 31) / 32, share = ((words + ctas - 1) / ctas + 1) / 2 * 64;
   const bool keep = share <= kMostKeys;
-  const int64_t smem = (ctas > 1 ? 6 : 3) * kBins * 4 + share / 4 + (keep ? share * 4 : 0);
+  const int64_t smem = (kBins + (ctas > 1 ? 3 * (kBins / ctas) : 0)) * 4 + share / 4 + (keep ? share * 4 : 0);
   static std::atomic<uint64_t> done[3][2];
   // long shares have more threads, many short ones more CTAs per SM
   const int which = !keep ? 2 : share > 4608 ? 1 : 0;
