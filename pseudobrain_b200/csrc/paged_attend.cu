@@ -24,7 +24,6 @@ constexpr int kUnit = 16;           // entries per unit
 constexpr int kRing = 192 * 1024;   // staging bytes per CTA
 constexpr int kMinUnits = 2;        // units per warp below which fewer warps take part
 constexpr int kClusterUnits = 320;  // most units per CTA where a cluster takes a whole head
-constexpr int kJoinThreads = 256;
 constexpr int kMassThreads = 256;
 constexpr int kPad = 4;             // floats after a partial row's D values: maximum, sum, two unused
 
@@ -630,7 +629,7 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     s_joined[tid] = make_float2(top, sum);
   }
   // this CTA's warps wrote the scores of its own units; its threads add their weights
-  const int h = c.pair;
+  const int h = c.pair, j0 = h * a.groups;
   int first_quarter = 0, end_quarter = 0;
   Quarter quarter;
   if (a.accumulate) {
@@ -649,14 +648,14 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
       sum += remote(&s_joined[row].y, k) * f;
       y += remote(&joined[i], k) * f;
     }
-    store_out<F16>(a, c.b * a.out_sb + (h * a.groups + row) * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
+    store_out<F16>(a, c.b * a.out_sb + (j0 + row) * a.out_sh + d, sum == 0.f ? 0.f : y * (1.f / sum));
   }
   if (tid < rows) {
     float top = -INFINITY, sum = 0.f;
     for (uint32_t k = 0; k < ctas; ++k) top = fmaxf(top, remote(&s_joined[tid].x, k));
     for (uint32_t k = 0; k < ctas; ++k) sum += remote(&s_joined[tid].y, k) * ex2(remote(&s_joined[tid].x, k) - finite(top));
     const float lse2 = finite(top) - a.offset + log2f(sum);
-    if (rank == 0) a.lse[(int64_t)c.b * a.kv * a.groups + h * a.groups + tid] = lse2 * kLn2;
+    if (rank == 0) a.lse[(int64_t)c.b * a.kv * a.groups + j0 + tid] = lse2 * kLn2;
     s_lse[tid] = lse2 == -INFINITY ? INFINITY : lse2;  // a row without weight adds 0
   }
   cluster_sync();  // no CTA leaves while another reads its part
@@ -672,11 +671,13 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
 // row's pieces (the first run's in its slot 1, the others' in slot 0), rescale as they go and
 // meet in shared memory. Where there are fewer query heads than runs (few sequences, many pieces
 // each) block i takes query head i, all warps on its one row; else (many sequences, few pieces)
-// block i looks at run i and takes the key head that it begins and does not end, if any.
-template <int D, bool F16>
-__global__ void __launch_bounds__(kJoinThreads)
+// block i looks at run i and takes the key head that it begins and does not end, if any. Blocks of
+// 1024 threads where the query heads are few enough to have an SM each: one long sequence of one
+// key head leaves several hundred pieces a head.
+template <int D, bool F16, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     paged_join_kernel(const AttendArgs a, int nwarps, bool by_head) {
-  constexpr int kWarps = kJoinThreads / 32;
+  constexpr int kWarps = THREADS / 32;
   constexpr int kEach = 4;  // pieces in flight per warp
   __shared__ float s_o[kWarps][D];
   __shared__ float s_ml[kWarps][2];
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int64_t total = a.base[a.batch] * (a.kv * a.rt);
     const int64_t u = a.base[b] * (a.kv * a.rt) + (int64_t)(h * a.rt + g / a.rows) * s.units;
     if (s.units == 0) {
-      for (int d = tid; d < D; d += kJoinThreads) store_out<F16>(a, b * a.out_sb + j * a.out_sh + d, 0.f);
+      for (int d = tid; d < D; d += THREADS) store_out<F16>(a, b * a.out_sb + j * a.out_sh + d, 0.f);
       if (tid == 0) a.lse[(int64_t)b * a.kv * a.groups + j] = -INFINITY;
       return;
     }
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     const int4 open = a.open[run];
     for (b = run; b < a.batch; b += gridDim.x)  // a sequence without entries is in no run
       if (Span(a, b).units == 0)
-        for (int i = tid; i < a.kv * a.groups * D; i += kJoinThreads) {
+        for (int i = tid; i < a.kv * a.groups * D; i += THREADS) {
           store_out<F16>(a, b * a.out_sb + i / D * a.out_sh + i % D, 0.f);
           if (i % D == 0) a.lse[(int64_t)b * a.kv * a.groups + i / D] = -INFINITY;
         }
@@ -748,7 +749,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     for (int e = 0; e < D / 32; ++e) s_o[warp][32 * e + lane] = acc[e];
     if (lane == 0) s_ml[warp][0] = top, s_ml[warp][1] = sum;
     __syncthreads();
-    for (int i = tid; i < n * D; i += kJoinThreads) {
+    for (int i = tid; i < n * D; i += THREADS) {
       const int r = i / D, d = i % D, j = h * a.groups + r0 + row0 + r;
       top = -INFINITY;
       for (int w = r * each; w < (r + 1) * each; ++w) top = fmaxf(top, s_ml[w][0]);
@@ -837,7 +838,9 @@ int clusters_at_once(int log_size) {
 // and clusters: 51 and 45 us; 96 heads: 42 and 36 us; with lengths spread over 1 .. 4000: 33 and
 // 34, 30 and 33 us). The cluster is the largest that leaves every warp two units. A CTA alone reads
 // some 75 GB/s, so that clusters on few of the SMs fall behind earlier (16 heads of 16000 entries on
-// 64 CTAs: 34 us; the runs take 21 us for lengths spread over 1 .. 16000).
+// 64 CTAs: 34 us; the runs take 21 us for lengths spread over 1 .. 16000). Heads of
+// several row tiles take the runs: two clusters would add to the same mass, and asking for the
+// weights is not to change a result's bits.
 int head_cluster(int64_t heads, int64_t units_per_head, int row_tiles) {
   if (row_tiles > 1 || heads > paged_sm_count()) return -1;
   int c = 0;
@@ -907,8 +910,10 @@ cudaError_t launch(const AttendArgs& a, const Plan& p, const CUtensorMap& mk, co
   if (e != cudaSuccess) return e;
   const int64_t query_heads = (int64_t)a.batch * a.kv * a.groups;
   const bool by_head = query_heads <= p.runs;
-  const cudaError_t j = launch_after(paged_join_kernel<D, F16>, dim3((unsigned)(by_head ? query_heads : p.runs)),
-                                     dim3(kJoinThreads), 0, st, 1, a, p.runs, by_head);
+  const dim3 grid((unsigned)(by_head ? query_heads : p.runs));
+  const cudaError_t j = by_head && query_heads <= paged_sm_count()
+                            ? launch_after(paged_join_kernel<D, F16, 1024>, grid, dim3(1024), 0, st, 1, a, p.runs, by_head)
+                            : launch_after(paged_join_kernel<D, F16, 256>, grid, dim3(256), 0, st, 1, a, p.runs, by_head);
   if (j != cudaSuccess || !a.accumulate || p.units_per_head == 0) return j;
   const int64_t slices = (p.units_per_head * 4 + kMassThreads - 1) / kMassThreads;
   return launch_after(paged_mass_kernel,
