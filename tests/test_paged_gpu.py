@@ -593,3 +593,21 @@ def test_a_pool_without_pages_and_a_table_without_columns(cuda_device, batch):
         src, dst, count = P.select_evictions(cache, table, lens, lens, 8)
         assert bool((count == 0).all()) and bool((src == -1).all()) and bool((dst == -1).all())
         assert bool((cache.mass == 0).all())
+
+
+@pytest.mark.parametrize("d,h", [(64, 4), (128, 4), (128, 16), (256, 6)])
+def test_attend_long_runs_do_not_lose_their_sum(cuda_device, d, h):
+    """1200 sequences over the same 131072 entries, so that a warp walks some 8192 units of a head:
+    with values of 1 the result is 1. The weights in two bf16 numbers are within 2^-16; each unit's
+    addition rounds by at most 2^-24 of the sum so far, either way, which in 8192 steps is
+    2^-24 sqrt(8192 / 3) / sqrt(3) at one standard deviation, 1.1e-5 < 2^-16 at six."""
+    from pseudobrain_b200.paged_cache import PagedCache, paged_attend
+    n, page, b = 131072, 64, 1200
+    g = torch.Generator(device=cuda_device).manual_seed(d + h)
+    k = torch.randn(n // page, 1, page, d, generator=g, device=cuda_device).to(torch.bfloat16)
+    cache = PagedCache(k, torch.ones_like(k))
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda_device)[None].expand(b, -1)
+    lens = torch.full((b,), n, dtype=torch.int32, device=cuda_device)
+    q = torch.randn(b, h, d, generator=g, device=cuda_device).to(torch.bfloat16)
+    out, _ = paged_attend(cache, q, table, lens, out=torch.empty(b, h, d, device=cuda_device))
+    assert float((out - 1).abs().max()) <= 2.0 ** -15
