@@ -108,6 +108,10 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+template <bool F16>
+__device__ __forceinline__ float round16(float x) {
+  return F16 ? __half2float(__float2half_rn(x)) : __bfloat162float(__float2bfloat16_rn(x));
+}
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -256,9 +260,11 @@ __device__ __forceinline__ float remote(const float* p, uint32_t rank) {
 // always towards zero; now that is 1e-5 at most, and nothing got slower but heads of 256 with more
 // than 8 rows (24 x 4 x 8000 entries, 16 rows: 106 -> 116 us in bf16, 105 -> 107 in fp16).
 //
-// Weights enter the product with V as 16-bit numbers: fp16 as one (11 bits), bf16 as two (the
-// rounded weight and what the rounding left, 16 bits together), so that the result's own
-// rounding is the largest error; the second product runs in the tensor cores' idle time.
+// Weights enter the product with V as two 16-bit numbers, the rounded weight and what the
+// rounding left (16 bits together in bf16, 22 in fp16), so that a 16-bit result's own rounding is
+// the largest error. The second product runs in the tensor cores' idle time where there are at most
+// 8 rows and the heads are no longer than 128; fp16 heads of 256 pay for it (window case 54.7 ->
+// 57.9 us, 24 x 4 x 8000 entries of 16 rows 107 -> 114).
 template <int D, int NT, bool F16, bool WHOLE>
 __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     paged_attend_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -505,12 +511,10 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
       for (int r = 0; r < 2; ++r) l[nt][r] = l[nt][r] * fac[nt][r] + (pr[r] + pr[2 + r]);
       pb[nt][0] = movmatrix_t(pack16<F16>(pr[0], pr[1]));
       pb[nt][1] = movmatrix_t(pack16<F16>(pr[2], pr[3]));
-      if (!F16) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] -= __bfloat162float(__float2bfloat16_rn(pr[e]));
-        pl[nt][0] = movmatrix_t(pack16<F16>(pr[0], pr[1]));
-        pl[nt][1] = movmatrix_t(pack16<F16>(pr[2], pr[3]));
-      }
+      for (int e = 0; e < 4; ++e) pr[e] -= round16<F16>(pr[e]);
+      pl[nt][0] = movmatrix_t(pack16<F16>(pr[0], pr[1]));
+      pl[nt][1] = movmatrix_t(pack16<F16>(pr[2], pr[3]));
     }
     if (a.accumulate) {
       float* to = a.scores + (u0 + i) * (int64_t)(kUnit * a.rows) + g;
@@ -531,7 +535,7 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
       for (int nt = 0; nt < NT; ++nt) {
         float unit[4] = {0.f, 0.f, 0.f, 0.f};
         mma16<F16>(unit, x0, x1, x2, x3, pb[nt][0], pb[nt][1]);
-        if (!F16) mma16<F16>(unit, x0, x1, x2, x3, pl[nt][0], pl[nt][1]);
+        mma16<F16>(unit, x0, x1, x2, x3, pl[nt][0], pl[nt][1]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][kk][e] = o[nt][kk][e] * fac[nt][e & 1] + unit[e];
       }

@@ -198,8 +198,9 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
     sequence (the token's own among them), of which the first ``sinks`` and the last ``window``
     are visible (all when window is None; entries count, so a window is for a cache whose
     entries lie in order). Returns out [B, H, hd] in q's dtype (or ``out``, which may be fp32)
-    and lse [B, H], the natural logarithm of the sum of exponentials. A sequence without
-    entries gives 0 and -inf. ``accumulate`` adds every entry's weight, summed over the query
+    and lse [B, H], the natural logarithm of the sum of exponentials. Scores and sums are fp32;
+    weights meet the values with 16 bits (bf16 caches) or 22 (fp16 caches), so an fp32 ``out``
+    holds about 5 or 6 digits. A sequence without entries gives 0 and -inf. ``accumulate`` adds every entry's weight, summed over the query
     heads of its key head, to cache.mass."""
     _need(cache, "paged_attend", "k_pages")
     if accumulate:

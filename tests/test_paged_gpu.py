@@ -611,3 +611,25 @@ def test_attend_long_runs_do_not_lose_their_sum(cuda_device, d, h):
     q = torch.randn(b, h, d, generator=g, device=cuda_device).to(torch.bfloat16)
     out, _ = paged_attend(cache, q, table, lens, out=torch.empty(b, h, d, device=cuda_device))
     assert float((out - 1).abs().max()) <= 2.0 ** -15
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,h,d", [(1, 1, 64), (1, 12, 128), (2, 5, 256), (300, 1, 64), (300, 12, 256), (300, 33, 128)])
+def test_attend_weights_have_both_their_16_bit_numbers(cuda_device, b, h, d, dtype):
+    """Entry e scores -4 e / d exactly and its value is 1 at place e, so out[e] is its weight. In
+    fp32 arithmetic the exponent errs by less than 6 (2^-24 + 2^-25) + 14 * 2^-24 < 1.4e-6, the
+    weight by ln 2 of that and 2^-22 for the power, their sum by as much again and the division by
+    2^-23: less than 2^-18 in all. Held in two numbers, a weight has 2^-16 (bf16) or 2^-22 (fp16)."""
+    from pseudobrain_b200.paged_cache import PagedCache, paged_attend
+    page = 16
+    e = torch.arange(d, device=cuda_device)
+    k = (-e.float())[:, None].expand(d, d).to(dtype).view(d // page, 1, page, d).contiguous()
+    v = torch.eye(d, device=cuda_device, dtype=dtype).view(d // page, 1, page, d)
+    table = torch.arange(d // page, dtype=torch.int32, device=cuda_device)[None].expand(b, -1)
+    lens = torch.full((b,), d, dtype=torch.int32, device=cuda_device)
+    q = torch.ones(b, h, d, dtype=dtype, device=cuda_device)
+    out, lse = paged_attend(PagedCache(k, v), q, table, lens, scale=4 / d ** 2, out=torch.empty(b, h, d, device=cuda_device))
+    x = -4 * e.double() / d
+    want = torch.softmax(x, -1)
+    assert float((out.double() / want - 1).abs().max()) <= (2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -22) + 2.0 ** -18
+    assert float((lse.double() - torch.logsumexp(x, -1)).abs().max()) <= 2.0 ** -18
