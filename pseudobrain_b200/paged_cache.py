@@ -157,8 +157,14 @@ def _rows(t: torch.Tensor, cache: PagedCache, what: str) -> None:
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _run(cache: PagedCache, fn, what: str, nbytes: int, *args) -> None:
-    """_call with a workspace of nbytes from the caching allocator behind the other arguments."""
+def _run(cache: PagedCache, fn, workspace, what: str, *args) -> None:
+    """_call with a workspace of workspace(*args) bytes from the caching allocator behind the other
+    arguments. Its size follows the current device's SMs and the clusters that it holds, so it is
+    asked for where the call will run."""
+    if not cache._only_gpu and torch.cuda.current_device() != cache._index:
+        with torch.cuda.device(cache._index):
+            return _run(cache, fn, workspace, what, *args)
+    nbytes = workspace(*args)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=cache.device)
         _call(cache, fn, what, *args, ws.data_ptr(), nbytes)
@@ -224,9 +230,7 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
     desc = PbkPagedAttendDesc(h, 0 if window is None else min(window, _INT_MAX), min(sinks, _INT_MAX), accumulate,
                               d ** -0.5 if scale is None else scale, dtype, q.data_ptr(), sb, sh, out.data_ptr(), ob, oh,
                               lse.data_ptr())
-    bref, dref = _byref(b), _byref(desc)
-    _run(cache, LIB.pbk_paged_attend, "pbk_paged_attend", LIB.pbk_paged_attend_workspace(cache._ref, bref, dref),
-         cache._ref, bref, dref)
+    _run(cache, LIB.pbk_paged_attend, LIB.pbk_paged_attend_workspace, "pbk_paged_attend", cache._ref, _byref(b), _byref(desc))
     return out, lse
 
 
@@ -244,9 +248,8 @@ def paged_observe_(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor
         raise ValueError(f"paged_observe_: q must be [{b.batch}, W, H, hd], got {tuple(q.shape)}")
     desc = PbkPagedObserveDesc(q.shape[2], q.shape[1], q.shape[3] ** -0.5 if scale is None else scale, 0, q.data_ptr(),
                                q.stride(0), q.stride(1), q.stride(2))
-    bref, dref = _byref(b), _byref(desc)
-    _run(cache, LIB.pbk_paged_observe, "pbk_paged_observe", LIB.pbk_paged_observe_workspace(cache._ref, bref, dref),
-         cache._ref, bref, dref)
+    _run(cache, LIB.pbk_paged_observe, LIB.pbk_paged_observe_workspace, "pbk_paged_observe", cache._ref, _byref(b),
+         _byref(desc))
 
 
 def select_evictions(cache: PagedCache, block_table: torch.Tensor, lengths: torch.Tensor, seen: torch.Tensor,

@@ -132,3 +132,44 @@ def test_oracle_attention_is_the_last_row_of_the_window_oracle(window, sinks):
     assert np.allclose([x.sum() for x in w], h)
     if window is None:
         assert np.allclose(op.observe(q[:, :, -1:].transpose(0, 2, 1, 3), kp, table, [n, n]), w, atol=1e-12)
+
+
+def test_workspaces_are_sized_on_the_caches_device(capi, monkeypatch):
+    """A cache on another device than the current one: the workspace's size, which follows the
+    device's SMs and clusters, and the launch are asked for with the cache's device current."""
+    import contextlib
+    import types
+
+    import torch
+    from pseudobrain_b200 import paged_cache as P
+    here, seen = [3], []
+
+    @contextlib.contextmanager
+    def device(i):
+        here[0], was = i, here[0]
+        yield
+        here[0] = was
+
+    def size(*args):
+        seen.append(("size", here[0]))
+        return 256
+
+    def launch(*args):
+        seen.append(("launch", here[0]))
+        return 0
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: here[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    monkeypatch.setattr(P, "LIB", types.SimpleNamespace(
+        pbk_paged_attend=launch, pbk_paged_attend_workspace=size, pbk_paged_observe=launch, pbk_paged_observe_workspace=size))
+    cache = object.__new__(P.PagedCache)  # host tensors stand for the device's: their device index is -1
+    cache.k_pages = cache.v_pages = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    cache.mass, cache.pos = torch.zeros(4, 2, 16), None
+    cache.device, cache._index, cache._only_gpu = torch.device("cpu"), -1, False
+    cache._desc = _cache(capi, d=64)
+    cache._ref = ctypes.byref(cache._desc)
+    q, table, lens = torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    P.paged_attend(cache, q, table, lens)
+    P.paged_observe_(cache, q[:, None], table, lens)
+    assert seen == [("size", -1), ("launch", -1)] * 2 and here == [3]
