@@ -32,7 +32,8 @@ with the table, lengths and seen shared by all layers (each layer has a pool of 
 of a page past a sequence's length may hold anything; page ids outside the pool are never
 followed. A page belongs to one sequence where a call writes it; attention without
 ``accumulate`` may read pages that several sequences share. Every kernel is CUDA (libpbk.so,
-sm_100a); there is no CPU path.
+sm_100a); there is no CPU path, and no call has a backward pass: the attention refuses a query
+that requires grad while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -209,6 +210,8 @@ def paged_attend(cache: PagedCache, q: torch.Tensor, block_table: torch.Tensor, 
     holds about 5 or 6 digits. A sequence without entries gives 0 and -inf. ``accumulate`` adds every entry's weight, summed over the query
     heads of its key head, to cache.mass."""
     _need(cache, "paged_attend", "k_pages")
+    if torch.is_grad_enabled() and (q.requires_grad or cache.k_pages.requires_grad or cache.v_pages.requires_grad):
+        raise RuntimeError("paged_attend has no backward pass: call it under torch.no_grad() or on detached tensors")
     if accumulate:
         _need(cache, "paged_attend", "mass")
     _rows(q, cache, "q")

@@ -134,6 +134,21 @@ def test_oracle_attention_is_the_last_row_of_the_window_oracle(window, sinks):
         assert np.allclose(op.observe(q[:, :, -1:].transpose(0, 2, 1, 3), kp, table, [n, n]), w, atol=1e-12)
 
 
+def _host_cache(capi):
+    """Host tensors in the place of the device's (their device index is -1), for what is decided in
+    Python: (cache, q, table, lengths)."""
+    import torch
+    from pseudobrain_b200 import paged_cache as P
+    cache = object.__new__(P.PagedCache)
+    cache.k_pages = cache.v_pages = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    cache.mass, cache.pos = torch.zeros(4, 2, 16), None
+    cache.device, cache._index, cache._only_gpu = torch.device("cpu"), -1, False
+    cache._desc = _cache(capi, d=64)
+    cache._ref = ctypes.byref(cache._desc)
+    return (cache, torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 1, dtype=torch.int32),
+            torch.zeros(3, dtype=torch.int32))
+
+
 def test_workspaces_are_sized_on_the_caches_device(capi, monkeypatch):
     """A cache on another device than the current one: the workspace's size, which follows the
     device's SMs and clusters, and the launch are asked for with the cache's device current."""
@@ -163,13 +178,32 @@ def test_workspaces_are_sized_on_the_caches_device(capi, monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
     monkeypatch.setattr(P, "LIB", types.SimpleNamespace(
         pbk_paged_attend=launch, pbk_paged_attend_workspace=size, pbk_paged_observe=launch, pbk_paged_observe_workspace=size))
-    cache = object.__new__(P.PagedCache)  # host tensors stand for the device's: their device index is -1
-    cache.k_pages = cache.v_pages = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
-    cache.mass, cache.pos = torch.zeros(4, 2, 16), None
-    cache.device, cache._index, cache._only_gpu = torch.device("cpu"), -1, False
-    cache._desc = _cache(capi, d=64)
-    cache._ref = ctypes.byref(cache._desc)
-    q, table, lens = torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    cache, q, table, lens = _host_cache(capi)
     P.paged_attend(cache, q, table, lens)
     P.paged_observe_(cache, q[:, None], table, lens)
     assert seen == [("size", -1), ("launch", -1)] * 2 and here == [3]
+
+
+def test_attention_refuses_to_lose_a_gradient(capi, monkeypatch):
+    """A query or a pool that requires grad is refused while gradients are recorded, not answered
+    with a result that has none; without recording the call runs."""
+    import types
+
+    import torch
+    from pseudobrain_b200 import paged_cache as P
+    calls = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    monkeypatch.setattr(P, "LIB", types.SimpleNamespace(pbk_paged_attend=lambda *a: calls.append(a) or 0,
+                                                        pbk_paged_attend_workspace=lambda *a: 0))
+    cache, q, table, lens = _host_cache(capi)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        P.paged_attend(cache, q.requires_grad_(), table, lens)
+    assert not calls
+    with torch.no_grad():
+        P.paged_attend(cache, q, table, lens)
+    P.paged_attend(cache, q.detach(), table, lens)
+    cache.k_pages = cache.k_pages.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        P.paged_attend(cache, q.detach(), table, lens)
+    assert len(calls) == 2
