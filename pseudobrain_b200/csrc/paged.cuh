@@ -14,6 +14,26 @@
 
 namespace pbk {
 
+namespace paged {
+
+// A ring of `stages` buffers, each with a barrier whose phase ends when a unit's copy has landed:
+// unit u lies in stage u % stages and ends its (u / stages)-th phase, so this is the parity to wait
+// for. A reader that gives up at unit i waits for the units i .. ring_issued(i, ...) - 1 before the
+// buffers are left: those that were issued (a unit is issued when the one `stages` before it has
+// been read) and not read.
+struct RingWait {
+  int stage;
+  uint32_t parity;
+};
+__host__ __device__ inline RingWait ring_wait(int64_t u, int stages) {
+  return {(int)(u % stages), (uint32_t)(u / stages & 1)};
+}
+__host__ __device__ inline int64_t ring_issued(int64_t i, int stages, int64_t count) {
+  return i + stages < count ? i + stages : count;
+}
+
+}  // namespace paged
+
 #ifdef __CUDACC__
 namespace paged {
 

@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
   int stage = 0;
   uint32_t parity = 0;
 
-  for (int i = 0; i < count; ++i) {
+  int i = 0;
+  for (; i < count; ++i) {
     const int h = c.pair / a.rt, r0 = (c.pair % a.rt) * a.rows;
     if (fresh) {
       fresh = false;
@@ -592,7 +593,10 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
     advance(c);
   }
   if (!ok)  // loads in flight land before the CTA's shared memory is given up
-    for (int s = 0; s < S::kStages; ++s) tc::mbar_wait(&s_full[warp][s], parity, 200000000ull);
+    for (int64_t u = i; u < paged::ring_issued(i, S::kStages, count); ++u) {
+      const paged::RingWait w = paged::ring_wait(u, S::kStages);
+      tc::mbar_wait(&s_full[warp][w.stage], w.parity, 200000000ull);
+    }
   if (!WHOLE) return;
 
   // ---- WHOLE: the warps' parts, each in its own (now free) ring, joined by the CTA into the

@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto load_queries = [&](int b, int h, int rt) -> bool {
       const uint32_t s = qt % S::kQueries, r = qt / S::kQueries;
-      ++qt;
       if (r > 0 && !__all_sync(0xffffffffu, wait(&q_empty[s], (r - 1) & 1, 1))) return false;
+      ++qt;
       if (lane == 0) {
         tc::mbar_expect_tx(&q_full[s], a.nw * a.groups * D * 2);
         for (int i = 0; i < D / 64; ++i)
@@ -292,11 +292,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (i + 1 < head.count) id = page_id(head, head.t + i + 1);
         else if (run.left > 0) id = page_id(run, run.t);
         const uint32_t s = kt % S::kKeys, r = kt / S::kKeys;
-        ++kt;
         if (r > 0 && !__all_sync(0xffffffffu, wait(&k_empty[s], (r - 1) & 1, 2))) {
           ok = false;
           break;
         }
+        ++kt;
         // (another producer's boxes may land first: the phase ends only after this arrival)
         if (producer == 0 && lane == 0) tc::mbar_expect_tx(&k_full[s], S::kBytes);
         if (mine)
@@ -305,12 +305,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int rt = 0; ok && !ONE && producer == 0 && rt < a.tiles; ++rt) ok = load_queries(head.b, head.h, rt);
       }
     }
-    // the loads issued here land before the CTA's shared memory is given up
-    if (producer == 0 && lane == 0) {
-      for (uint32_t i = kt > S::kKeys ? kt - S::kKeys : 0; i < kt; ++i)
-        tc::mbar_wait(&k_full[i % S::kKeys], (i / S::kKeys) & 1, 200000000ull);
-      for (uint32_t i = qt > S::kQueries ? qt - S::kQueries : 0; i < qt; ++i)
-        tc::mbar_wait(&q_full[i % S::kQueries], (i / S::kQueries) & 1, 200000000ull);
+    // the loads issued here land before the CTA's shared memory is given up (a key tile's phase ends
+    // when both producers' have)
+    if (lane == 0) {
+      for (uint32_t i = kt > S::kKeys ? kt - S::kKeys : 0; i < kt; ++i) {
+        const paged::RingWait w = paged::ring_wait(i, S::kKeys);
+        tc::mbar_wait(&k_full[w.stage], w.parity, 200000000ull);
+      }
+      for (uint32_t i = qt > S::kQueries ? qt - S::kQueries : 0; i < qt; ++i) {
+        const paged::RingWait w = paged::ring_wait(i, S::kQueries);
+        tc::mbar_wait(&q_full[w.stage], w.parity, 200000000ull);
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer

@@ -207,3 +207,49 @@ def test_attention_refuses_to_lose_a_gradient(capi, monkeypatch):
     with pytest.raises(RuntimeError, match="no backward pass"):
         P.paged_attend(cache, q.detach(), table, lens)
     assert len(calls) == 2
+
+
+def test_a_ring_that_is_left_early_waits_for_every_copy_in_flight():
+    """The waits of a reader that gives up, on a model of the ring's barriers: for every ring, number of
+    units and place to stop, each unit issued and not read is waited for, and its wait ends with its
+    own copy and not before."""
+    src = """
+    #include <stdio.h>
+    #include <vector>
+    #include "paged.cuh"
+    using namespace pbk::paged;
+    int main() {
+      long bad = 0, seen = 0;
+      for (int stages = 1; stages <= 6; ++stages)
+        for (int count = 0; count <= 40; ++count)
+          for (int stop = 0; stop < count; ++stop) {
+            std::vector<long> ended(stages, 0);  // phases of each stage's barrier that have ended
+            auto open = [&](RingWait w) { return (ended[w.stage] & 1) == w.parity; };  // a wait would block
+            long issued = count < stages ? count : stages;
+            for (int u = 0; u < stop; ++u) {  // read, and the stage filled again
+              if (!open(ring_wait(u, stages))) ++bad;
+              ++ended[u % stages];
+              if (open(ring_wait(u, stages))) ++bad;
+              if (u + stages < count) ++issued;
+            }
+            if (ring_issued(stop, stages, count) != issued) ++bad;
+            for (long u = stop; u < issued; ++u) {
+              ++seen;
+              if (!open(ring_wait(u, stages))) ++bad;  // would return with the copy in flight
+            }
+            for (long u = stop; u < issued; ++u) {
+              ++ended[u % stages];
+              if (open(ring_wait(u, stages))) ++bad;   // would wait for ever
+            }
+          }
+      printf("%ld %ld", bad, seen);
+    }
+    """
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = os.path.join(d, "ring.cpp"), os.path.join(d, "ring")
+        with open(c, "w") as f:
+            f.write(src)
+        subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "include"), "-I",
+                        os.path.join(ROOT, "pseudobrain_b200", "csrc"), "-I", "/usr/local/cuda/include", c, "-o", exe], check=True)
+        bad, seen = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()
+    assert bad == "0" and int(seen) > 10000
