@@ -633,3 +633,148 @@ def test_attend_weights_have_both_their_16_bit_numbers(cuda_device, b, h, d, dty
     want = torch.softmax(x, -1)
     assert float((out.double() / want - 1).abs().max()) <= (2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -22) + 2.0 ** -18
     assert float((lse.double() - torch.logsumexp(x, -1)).abs().max()) <= 2.0 ** -18
+
+
+def spread(seed, count, top, *first):
+    """`count` lengths: those given, then some from 0 to `top`."""
+    return (list(first) + np.random.default_rng(seed).integers(0, top + 1, count).tolist())[:count]
+
+
+RUNS = [
+    # lengths, h, kv, d, page, window, sinks: more units than a warp's ring holds, heads cut over runs
+    (spread(1, 40, 3000, 3000, 0, 1, 0), 32, 8, 64, 16, None, 0),     # joined by runs (1280 query heads, 1184 runs)
+    (spread(2, 30, 1500, 1500, 0, 699, 700, 701, 740), 40, 8, 128, 8, 700, 37),    # window and sinks over runs
+    (spread(3, 40, 600, 600, 17), 24, 4, 256, 64, None, 0),           # 960 query heads, 888 runs
+    (spread(4, 30, 1500, 1400, 3), 96, 8, 64, 32, 260, 600),          # sinks up to the window
+    (spread(5, 160, 2000, 2000, 0, 16), 2, 1, 128, 32, None, 0),      # joined by heads on 256 threads
+    (spread(6, 160, 900, 900, 0, 16), 10, 1, 256, 8, 300, 4),         # the same, 10 rows, a window
+    ([30000], 4, 1, 256, 16, None, 0),                                # by heads on 1024 threads
+    ([60001], 12, 1, 64, 128, 31000, 100),
+    ([0, 41003, 5], 8, 2, 128, 8, None, 0),
+    (spread(7, 12, 9000, 9000, 0), 40, 2, 64, 16, None, 0),           # two row tiles of ten
+    (spread(8, 12, 4000, 4000), 66, 2, 128, 256, 2000, 33),           # three row tiles
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(RUNS)))
+def test_attend_by_equal_runs(cuda_device, case, dtype):
+    """The path of ragged batches and of long sequences. A workspace without weights to add says that
+    a call takes it (clusters need none)."""
+    from pseudobrain_b200 import _capi
+    from pseudobrain_b200 import paged_cache as P
+    lengths, h, kv, d, page, window, sinks = RUNS[case]
+    cache, table, lens, q = make(200 + case, lengths, h, kv, d, page, dtype, cuda_device)
+    desc = _capi.PbkPagedAttendDesc(h, window or 0, sinks, 0, 0.1, _capi.PBK_F32, 16, d, d, 16, d, d, 16)
+    assert P.LIB.pbk_paged_attend_workspace(cache._ref, P._batch(cache, table, lens), desc) > 0
+    before = _np(cache.mass)
+    out, lse = P.paged_attend(cache, q, table, lens, window, sinks)
+    check_attend(cache, table, lens, q, out, lse, before, window, sinks)
+    again = P.paged_attend(cache, q, table, lens, window, sinks, accumulate=True)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    check_attend(cache, table, lens, q, *again, before, window, sinks, accumulate=True)
+    assert _capi.device_error() == 0
+
+
+OBSERVE_RUNS = [
+    # lengths, w, h, kv, d, page, tiles per CTA: more key tiles per CTA than two turns of its ring
+    ([23000, 17003, 0, 12011, 7189], 32, 32, 8, 64, 8, 25),                 # 128 rows, long heads
+    (spread(21, 61, 2100, 2100, 1, 0, 19), 20, 24, 4, 128, 16, 13),         # 120 rows, heads of 0 to 17 tiles
+    ([30011, 3, 27000, 5000], 5, 6, 2, 256, 256, 6),                        # 15 rows
+    (spread(22, 700, 300, 300, 0, 1, 0), 7, 12, 4, 64, 16, 25),             # many heads of one to three tiles
+    ([60000, 45003, 20], 40, 16, 2, 64, 64, 11),                            # 3 row tiles
+    (spread(23, 70, 2000, 2000, 0, 49, 50, 51), 50, 12, 2, 128, 16, 7),     # 3 row tiles, a sequence as long as the queries
+    (spread(24, 40, 3900, 3900, 63, 0), 64, 6, 1, 256, 32, 4),              # 4 row tiles, one stage of keys
+    (spread(25, 30, 4000, 4000), 70, 24, 1, 64, 16, 3),                     # 14 row tiles: two launches a pass
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(OBSERVE_RUNS)))
+def test_observe_over_many_key_tiles(cuda_device, case, dtype):
+    """The pipeline at work: rings and accumulators in their second turns, runs over several heads and
+    sequences, heads over several runs."""
+    from pseudobrain_b200 import _capi
+    from pseudobrain_b200.paged_cache import paged_observe_
+    lengths, w, h, kv, d, page, each = OBSERVE_RUNS[case]
+    sms = torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    assert kv * sum(-(-n // 128) for n in lengths) > (each - 1) * sms
+    cache, table, lens, _ = make(300 + case, lengths, h, kv, d, page, dtype, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(case)
+    q = torch.randn(len(lengths), w, h, d, generator=g, device=cuda_device).to(dtype)
+    start, before = cache.mass.clone(), _np(cache.mass)
+    paged_observe_(cache, q, table, lens)
+    t = used_table(table, lengths, page)
+    want, slack = before.copy(), np.zeros_like(before)
+    for i, add in enumerate(op.observe(_np(q), _np(cache.k_pages), t, lengths)):
+        p, r = op.entry(t, page, i, np.arange(add.shape[1]))
+        for j in range(kv):
+            want[p, j, r] += add[j]
+            slack[p, j, r] += 2 * SCORE * add[j] + 2.0 ** -22 * want[p, j, r]
+    assert (np.abs(_np(cache.mass) - want) <= slack).all()
+    first = cache.mass.clone()
+    cache.mass.copy_(start)
+    paged_observe_(cache, q, table, lens)
+    assert torch.equal(cache.mass, first) and _capi.device_error() == 0
+
+
+def choose(mass, pos, seen, budget, recent, sinks):
+    """The moves (src, dst) of one row of n entries, by sorting."""
+    n = len(mass)
+    safe = ((pos >= 0) & (pos < sinks)) | (pos.astype(np.int64) >= seen - recent)
+    nan = np.isnan(mass) & ~safe
+    value = np.where(safe | nan, np.float32(0), mass)
+    order = np.lexsort((np.arange(n), -value, ~nan, ~safe))
+    kept = np.zeros(n, bool)
+    kept[order[:budget]] = True
+    at = np.arange(n)
+    return at[kept & (at >= budget)], at[~kept & (at < budget)]
+
+
+@pytest.mark.parametrize("lengths,kv,page,budget,recent,sinks,kind,width", [
+    ([131072], 8, 16, 4096, 512, 4, "weights", None),                     # 16 CTAs of 512 threads
+    ([131072], 2, 64, 130000, 3, 0, "near", None),                        # all three digits count
+    ([131072, 4097, 70001, 4096, 0], 3, 16, 4096, 512, 4, "five", None),  # ties, shorter than the shares
+    (spread(31, 25, 20000, 20000, 4099), 8, 16, 4096, 64, 4, "near", None),      # one CTA of 512 threads each
+    (spread(32, 25, 30000, 30000, 9000), 8, 32, 9000, 64, 4, "weights", None),   # clusters of two
+    ([24576, 24000], 80, 8, 12000, 0, 0, "five", None),                   # the longest share that is kept
+    ([24577, 100, 24576], 60, 8, 24000, 9, 9, "odd", None),
+    ([400003, 393217, 100], 2, 128, 4096, 512, 4, "weights", None),       # keys read again in every pass
+    ([400003, 25000], 1, 8, 300000, 0, 7, "five", None),
+    ([600001, 30], 2, 256, 100000, 1000, 4, "near", 1 << 15),             # a table of 2^23 entries
+    ([1 << 23], 1, 256, 1 << 20, 1 << 19, 4, "odd", None),                # the most that a row may hold
+])
+def test_select_of_long_rows_matches_sorting(cuda_device, lengths, kv, page, budget, recent, sinks, kind, width):
+    """Shares of over 4608 entries (512 threads) and of over 24576 (not kept in shared memory)."""
+    from pseudobrain_b200 import _capi
+    from pseudobrain_b200.paged_cache import PagedCache, select_evictions
+    rng = np.random.default_rng(sum(lengths) + budget)
+    n, b = max(lengths), len(lengths)
+    m = -(-n // page)
+    mass = {"weights": lambda: rng.random((b, kv, m * page), np.float32) ** 8 * 50,
+            "near": lambda: (1 + rng.integers(0, 3000, (b, kv, m * page)) * 2.0 ** -23).astype(np.float32),
+            "five": lambda: rng.integers(-1, 4, (b, kv, m * page)).astype(np.float32),
+            "odd": lambda: rng.standard_normal((b, kv, m * page), np.float32)}[kind]()
+    if kind == "odd":
+        mass[..., ::97], mass[..., 5::101], mass[..., 7::103], mass[..., 11::89] = np.nan, np.inf, -np.inf, -0.0
+    pos = rng.permuted(np.broadcast_to(np.arange(m * page, dtype=np.int32), mass.shape), axis=-1)
+    seen = np.asarray(lengths, np.int64) + 3
+    table = rng.permutation(b * m).reshape(b, m).astype(np.int32)
+    pools = [torch.zeros(b * m, kv, page, dtype=dt, device=cuda_device) for dt in (torch.float32, torch.int32)]
+    t = torch.from_numpy(table).long().to(cuda_device)
+    for pool, x in zip(pools, (mass, pos)):
+        pool[t] = torch.from_numpy(x).to(cuda_device).view(b, kv, m, page).transpose(1, 2)
+    wide = torch.full((b, width or m), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, :m] = t
+    dev = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device=cuda_device)  # noqa: E731
+    got = select_evictions(PagedCache(None, None, *pools), wide, dev(lengths), dev(seen), budget, recent, sinks)
+    src, dst, count = (x.cpu().numpy() for x in got)
+    assert src.shape[2] == dst.shape[2] == max(0, min(budget, (width or m) * page - budget))
+    for i, length in enumerate(lengths):
+        for j in range(kv):
+            s, d = choose(mass[i, j, :length], pos[i, j, :length], int(seen[i]), budget, recent, sinks) \
+                if length > budget else ([], [])
+            assert count[i, j] == len(s) == len(d)
+            assert np.array_equal(src[i, j, :len(s)], s) and np.array_equal(dst[i, j, :len(d)], d)
+            assert (src[i, j, len(s):] == -1).all() and (dst[i, j, len(d):] == -1).all()
+    assert _capi.device_error() == 0
