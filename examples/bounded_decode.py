@@ -5,9 +5,11 @@ layer's cache stays within its budget.
     python examples/bounded_decode.py [--batch 4] [--prompt 2000] [--tokens 128] [--budget 512]
 
 Every layer has a pool of pages; the block table, the lengths and the positions are shared by
-all of them. A decode step (append, attention with its weights, the projections) is one CUDA
-graph; an eviction, another, runs once per page of new tokens. Prints the time per step beside
-that of the whole cache, and how far the two streams of hidden states drift apart.
+all of them. Once the prompt is evicted, the calls get the columns of the table that a bounded
+sequence can use: their plans follow the table's width. A decode step (append, attention with its
+weights, the projections) is one CUDA graph; an eviction, another, runs once per page of new
+tokens. Prints the time per step beside that of the whole cache, and how far the two streams of
+hidden states drift apart.
 """
 from __future__ import annotations
 
@@ -63,6 +65,8 @@ class Decoder:
         self.a, self.budget = a, budget
         self.layers = [Layer(a.hidden, a.heads, a.kv, 128, a.batch * width, a.page, gen) for _ in range(a.layers)]
         self.table = torch.randperm(a.batch * width, generator=gen, device="cuda").to(torch.int32).view(a.batch, width)
+        # from the prompt's eviction on: the budget and the tokens until the next eviction
+        self.used = self.table if budget is None else self.table[:, : -(-(budget + a.page) // a.page)]
         self.lengths = torch.zeros(a.batch, dtype=torch.int32, device="cuda")
         self.after = torch.zeros_like(self.lengths)
         self.seen = torch.zeros_like(self.lengths)
@@ -75,19 +79,19 @@ class Decoder:
         self.lengths += self.a.prompt
         self.seen += self.a.prompt
         if self.budget:
-            self.evict()
+            self.evict(self.table)
         return x[:, -1].clone()
 
-    def evict(self) -> None:
+    def evict(self, table: torch.Tensor) -> None:
         for layer in self.layers:
-            paged_evict_(layer.cache, self.table, self.lengths, self.seen, self.budget, self.a.recent, self.a.sinks)
+            paged_evict_(layer.cache, table, self.lengths, self.seen, self.budget, self.a.recent, self.a.sinks)
         self.lengths.clamp_(max=self.budget)
 
     def step(self, x: torch.Tensor) -> None:
         y = x
         torch.add(self.lengths, 1, out=self.after)
         for layer in self.layers:
-            y = layer.step(y, self.table, self.lengths, self.seen, self.after, self.budget is not None)
+            y = layer.step(y, self.used, self.lengths, self.seen, self.after, self.budget is not None)
         x.copy_(y / y.float().square().mean(-1, keepdim=True).sqrt())
         self.lengths += 1
         self.seen += 1
@@ -108,7 +112,7 @@ class Decoder:
                 self.step(x)
             if self.budget:
                 with torch.cuda.graph(evict, stream=side):
-                    self.evict()
+                    self.evict(self.used)
             start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             start.record()
             for i in range(self.a.tokens):
