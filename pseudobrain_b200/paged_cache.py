@@ -54,6 +54,12 @@ _byref = ctypes.byref
 _INT_MAX = 2 ** 31 - 1
 
 
+def _same_places(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the elements of two tensors of one shape lie alike: the same strides, those of
+    dimensions of one element aside (they may be anything)."""
+    return a.stride() == b.stride() or all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
 @dataclass
 class PagedCache:
     """One layer's pool of pages: keys and values [P, KV, page, hd], and per entry and key head
@@ -79,7 +85,7 @@ class PagedCache:
             raise ValueError("paged cache: keys and values come together")
         if self.k_pages is not None:
             k, v = self.k_pages, self.v_pages
-            if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride():
+            if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or not _same_places(k, v):
                 raise ValueError("paged cache: k_pages and v_pages must be alike, [P, KV, page, hd]")
             if k.dtype not in (torch.bfloat16, torch.float16):
                 raise TypeError(f"paged cache: bf16 or fp16 keys and values expected, got {k.dtype}")
@@ -187,8 +193,8 @@ def paged_append_(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_tab
     _need(cache, "paged_append_", "k_pages")
     _rows(k, cache, "k")
     shape, strides = k.shape, k.stride()
-    if len(shape) != 3 or shape[1] != cache._desc.kv or v.shape != shape or v.dtype != k.dtype or v.stride() != strides \
-            or v.get_device() != cache._index:
+    if len(shape) != 3 or shape[1] != cache._desc.kv or v.shape != shape or v.dtype != k.dtype \
+            or not _same_places(k, v) or v.get_device() != cache._index:
         raise ValueError(f"paged_append_: k and v must be alike, [N, {cache.kv}, hd] with the same strides, got "
                          f"{tuple(k.shape)} {strides} and {tuple(v.shape)} {v.stride()}")
     b = _batch(cache, block_table, lengths, seen)

@@ -253,3 +253,24 @@ def test_a_ring_that_is_left_early_waits_for_every_copy_in_flight():
                         os.path.join(ROOT, "pseudobrain_b200", "csrc"), "-I", "/usr/local/cuda/include", c, "-o", exe], check=True)
         bad, seen = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()
     assert bad == "0" and int(seen) > 10000
+
+
+def test_append_takes_one_token_whose_key_and_value_rows_differ_in_stride(capi, monkeypatch):
+    """Of a single token the stride between tokens means nothing: a key of its own beside a value
+    inside a packed projection is taken; of two tokens it is refused."""
+    import types
+
+    import torch
+    from pseudobrain_b200 import paged_cache as P
+    calls = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    monkeypatch.setattr(P, "LIB", types.SimpleNamespace(pbk_paged_append=lambda *a: calls.append(a) or 0))
+    cache, _, table, lens = _host_cache(capi)
+    packed = torch.zeros(2, 12, 64, dtype=torch.bfloat16)
+    k, v = torch.zeros(2, 2, 64, dtype=torch.bfloat16), packed[:, 10:]
+    P.paged_append_(cache, k[:1], v[:1], table[:1], lens[:1])
+    assert calls[0][2:7] == (k.data_ptr(), v.data_ptr(), 128, 64, 1)
+    with pytest.raises(ValueError, match="same strides"):
+        P.paged_append_(cache, k, v, table[:2], lens[:2])
+    assert len(calls) == 1
